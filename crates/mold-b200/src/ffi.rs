@@ -32,6 +32,11 @@ pub const MB_DT_BF16: c_int = 1;
 pub const MB_EPI_NONE: c_int = 0;
 pub const MB_EPI_GELU_TANH: c_int = 1;
 pub const MB_EPI_GATE_RESIDUAL: c_int = 2;
+pub const MB_KV_BF16: c_int = 0;
+pub const MB_KV_I8: c_int = 1;
+pub const MB_KV_E4M3: c_int = 2;
+/// A device status (`mb_device_status`): a page table entry outside the cache.
+pub const MB_DEV_BAD_PAGE: c_int = 0x400;
 
 #[repr(C)]
 pub struct MbWeight {
@@ -84,6 +89,21 @@ pub struct MbInpaint {
     pub mask: *const f32,
     pub original: *const f32,
     pub noise: *const f32,
+}
+
+/// `mb_kv_cache`: a paged key-value cache in caller-owned device memory.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct MbKvCache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub n_pages: i64,
+    pub page_size: c_int,
+    pub n_kv_heads: c_int,
+    pub head_dim: c_int,
+    pub dtype: c_int,
 }
 
 /// `mb_step_callback`: runs on a CUDA host-function thread after each finished step; it must
@@ -218,5 +238,28 @@ extern "C" {
     pub fn mb_flux_lora_merge(
         m: *mut MbFlux, name: *const c_char, row_offset: i64, rows: i64, a: *const f32, b: *const f32,
         rank: c_int, scale: f32, stream: *mut c_void,
+    ) -> MbStatus;
+    pub fn mb_attention_varlen(
+        q: *const c_void, ldq: i64, k: *const c_void, ldk: i64, v: *const c_void, ldv: i64, total_q: i64,
+        total_k: i64, h: c_int, h_kv: c_int, d: c_int, cu_q: *const i32, cu_k: *const i32, n_seqs: c_int,
+        causal: c_int, scale: f32, out: *mut c_void, ldo: i64, stream: *mut c_void,
+    ) -> MbStatus;
+    pub fn mb_kv_write(
+        cache: *const MbKvCache, k: *const c_void, ldk: i64, v: *const c_void, ldv: i64, n_tokens: i64,
+        cu: *const i32, kv_lens: *const i32, table: *const i32, ld_table: i64, table_width: c_int,
+        n_seqs: c_int, stream: *mut c_void,
+    ) -> MbStatus;
+    pub fn mb_kv_read(
+        cache: *const MbKvCache, cu: *const i32, table: *const i32, ld_table: i64, table_width: c_int,
+        n_seqs: c_int, n_tokens: i64, k: *mut c_void, ldk: i64, v: *mut c_void, ldv: i64,
+        stream: *mut c_void,
+    ) -> MbStatus;
+    pub fn mb_attention_paged_workspace(
+        n_seqs: c_int, h: c_int, h_kv: c_int, d: c_int, bytes: *mut usize,
+    ) -> MbStatus;
+    pub fn mb_attention_paged(
+        q: *const c_void, ldq: i64, cache: *const MbKvCache, kv_lens: *const i32, table: *const i32,
+        ld_table: i64, table_width: c_int, n_seqs: c_int, h: c_int, scale: f32, out: *mut c_void, ldo: i64,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void,
     ) -> MbStatus;
 }

@@ -396,6 +396,88 @@ MB_API mb_status mb_weight_lora_merge(mb_weight* w, int64_t row_offset, int64_t 
 MB_API mb_status mb_flux_lora_merge(mb_flux* m, const char* name, int64_t row_offset, int64_t rows, const float* A,
                                     const float* B, int rank, float scale, void* stream);
 
+/* ------------------------------------------------------------------ text transformers
+ *
+ * Attention of the causal text transformers whose hidden states condition the image models
+ * (grouped heads: query head h reads key head h / (H / H_kv)), over packed batches and over a
+ * paged key-value cache. No counterpart in the reference's denoising path, whose attention is
+ * one non-causal sequence a call (flux/offload.rs:40-54); its GGUF text encoders
+ * (encoders/qwen3_gguf.rs:273-305) run the same mathematics through candle products.
+ *
+ * Shared rules. q, k, v and out are bf16; row strides (ld*) are in elements, a row's heads are
+ * D apart; D is 64 or 128. `cu` arrays are device int32 [n_seqs + 1]: sequence b's rows are
+ * [cu[b], cu[b + 1]) of the packed tensor; rows from cu[n_seqs] on belong to nobody and are left
+ * as they were. Device-side indices are checked by the kernels: rows and pages outside the
+ * given sizes are neither read nor written, and a page number outside the cache that a call
+ * needed raises MB_DEV_BAD_PAGE in the device status word (mb_device_status). mb_init must have
+ * been called on the device (else MB_ERR_NOT_READY). Nothing is allocated; every call may be
+ * captured into a CUDA graph, and its scratch is the caller's. */
+
+enum { MB_DEV_BAD_PAGE = 0x400 };
+
+/* Element types of a key-value cache. */
+enum { MB_KV_BF16 = 0, MB_KV_I8 = 1, MB_KV_E4M3 = 2 };
+
+/* A paged cache in caller-owned device memory. k, v: [n_pages, n_kv_heads, page_size, head_dim]
+ * elements of `dtype`, 16-byte aligned; k_scale, v_scale: f32 [n_pages, n_kv_heads, page_size],
+ * 8-byte aligned (NULL for MB_KV_BF16). page_size: a power of two, 16 to 256. A sequence's
+ * position p lies in page table[b][p / page_size] at offset p % page_size (table: device int32,
+ * table_width pages of each sequence, rows ld_table apart); entries behind a sequence's last
+ * page are not read. */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t n_pages;
+  int page_size;
+  int n_kv_heads;
+  int head_dim;
+  int dtype;
+} mb_kv_cache;
+
+/* K11. Attention of packed prompts: sequence b has m = cu_q[b+1] - cu_q[b] queries (q bf16
+ * [total_q, H, D]) and n = cu_k[b+1] - cu_k[b] keys (k, v bf16 [total_k, H_kv, D]), and
+ *   out[i, h] = sum_j w_ij v[j, h'],  w = softmax over j of scale * q[i, h] . k[j, h'],
+ * over all n keys, or with `causal` over j <= i + n - m (the queries are the last m positions).
+ * A row that its mask leaves no key is 0. scale > 0; 0 stands for 1 / sqrt(D). What is not
+ * finite in keys that a row's mask leaves out does not reach the row. */
+MB_API mb_status mb_attention_varlen(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                                     int64_t ldv, int64_t total_q, int64_t total_k, int H, int H_kv, int D,
+                                     const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int causal, float scale,
+                                     void* out, int64_t ldo, void* stream);
+
+/* K12. Append to the cache: sequence b's rows of k, v (bf16 [n_tokens, n_kv_heads, head_dim]) go
+ * to its last positions, kv_lens[b] - m .. kv_lens[b] - 1 (kv_lens: device int32, the lengths
+ * after the call). cu NULL: one row each (n_tokens == n_seqs); a sequence with kv_lens[b] <= 0
+ * is passed over. MB_KV_BF16 keeps the values. The 8-bit types keep for each row of head_dim
+ * values x the scale s = max|x| / T and the codes c nearest to x * (T / max|x|), ties to even
+ * (scale, inverse and product rounded to f32; T = 127 or 448), standing for c * s. A row whose
+ * largest magnitude is below 2^-100 is stored as zeros; one with a NaN or infinity reads back
+ * as NaN. A position is to be written once in a call: of two rows for one place (a page in two
+ * table rows) either may stay, in part. */
+MB_API mb_status mb_kv_write(const mb_kv_cache* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                             int64_t n_tokens, const int32_t* cu, const int32_t* kv_lens, const int32_t* table,
+                             int64_t ld_table, int table_width, int n_seqs, void* stream);
+
+/* K13. Read the cache back: row cu[b] + p of k, v (bf16 [n_tokens, n_kv_heads, head_dim]) =
+ * position p of sequence b, for its first cu[b+1] - cu[b] positions (the keys of
+ * mb_attention_varlen for the next piece of a prompt). A position without a page reads as 0. */
+MB_API mb_status mb_kv_read(const mb_kv_cache* cache, const int32_t* cu, const int32_t* table, int64_t ld_table,
+                            int table_width, int n_seqs, int64_t n_tokens, void* k, int64_t ldk, void* v,
+                            int64_t ldv, void* stream);
+
+/* K14. Attention of one new token of each sequence over its cached positions 0 .. kv_lens[b] - 1
+ * (at most table_width * page_size): q bf16 [n_seqs, H, D], out bf16 likewise; a sequence without
+ * positions gives 0. The cached lengths are split over the SMs and the parts joined in a fixed
+ * order, so equal calls give equal bits. workspace: mb_attention_paged_workspace bytes of device
+ * memory, 16-byte aligned, that no other call uses meanwhile (its contents need no setup). */
+MB_API mb_status mb_attention_paged_workspace(int n_seqs, int H, int H_kv, int D, size_t* bytes);
+MB_API mb_status mb_attention_paged(const void* q, int64_t ldq, const mb_kv_cache* cache, const int32_t* kv_lens,
+                                    const int32_t* table, int64_t ld_table, int table_width, int n_seqs, int H,
+                                    float scale, void* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,8 @@ GGML_F32, GGML_F16, GGML_Q8_0, GGML_Q4_K, GGML_BF16 = 0, 1, 8, 12, 30
 GGML_Q4_0, GGML_Q4_1, GGML_Q5_0, GGML_Q5_1, GGML_Q5_K, GGML_Q6_K = 2, 3, 6, 7, 13, 14
 DT_F32, DT_BF16 = 0, 1
 EPI_NONE, EPI_GELU_TANH, EPI_GATE_RESIDUAL = 0, 1, 2
+KV_BF16, KV_I8, KV_E4M3 = 0, 1, 2
+DEV_BAD_PAGE = 0x400
 
 _STATUS_NAMES = {0: "MB_OK", 1: "MB_ERR_INVALID", 2: "MB_ERR_UNSUPPORTED", 3: "MB_ERR_CUDA", 4: "MB_ERR_TIMEOUT",
                  5: "MB_ERR_NOMEM", 6: "MB_ERR_NOT_READY"}
@@ -63,6 +65,11 @@ SIGNATURES = {
     "mb_qwen_load_gguf": (I32, [P, ctypes.c_char_p, P]),
     "mb_weight_lora_merge": (I32, [P, I64, I64, P, P, I32, F32, P]),
     "mb_flux_lora_merge": (I32, [P, ctypes.c_char_p, I64, I64, P, P, I32, F32, P]),
+    "mb_attention_varlen": (I32, [P, I64, P, I64, P, I64, I64, I64, I32, I32, I32, P, P, I32, I32, F32, P, I64, P]),
+    "mb_kv_write": (I32, [P, P, I64, P, I64, I64, P, P, P, I64, I32, I32, P]),
+    "mb_kv_read": (I32, [P, P, P, I64, I32, I32, I64, P, I64, P, I64, P]),
+    "mb_attention_paged_workspace": (I32, [I32, I32, I32, I32, P]),
+    "mb_attention_paged": (I32, [P, I64, P, P, P, I64, I32, I32, I32, F32, P, I64, P, SZ, P]),
 }
 
 
@@ -86,6 +93,11 @@ class QwenConfigC(ctypes.Structure):
     _fields_ = [("in_channels", I32), ("out_channels", I32), ("patch_size", I32), ("joint_attention_dim", I32),
                 ("hidden_size", I32), ("num_heads", I32), ("num_layers", I32), ("mlp_hidden", I32),
                 ("axes_dim", I32 * 3), ("theta", I32)]
+
+
+class KVCacheC(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("k_scale", P), ("v_scale", P), ("n_pages", I64), ("page_size", I32),
+                ("n_kv_heads", I32), ("head_dim", I32), ("dtype", I32)]
 
 
 _lib = None

@@ -21,6 +21,7 @@ enum DeviceStatus : int {
   kDevTimeoutGemm = 0x100,
   kDevTimeoutAttn = 0x200,
   kDevTimeoutGemv = 0x300,
+  kDevBadPage = 0x400,  // MB_DEV_BAD_PAGE
 };
 
 // ~2 s at 1.9 GHz: far above any legitimate wait of these kernels.

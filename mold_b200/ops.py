@@ -8,7 +8,7 @@ import ctypes
 import numpy as np
 import torch
 
-from ._lib import (STEP_CALLBACK, InpaintC, DT_BF16, DT_F32, EPI_GATE_RESIDUAL, EPI_GELU_TANH, EPI_NONE, GGML_BF16, GGML_F16, GGML_F32,
+from ._lib import (STEP_CALLBACK, InpaintC, KVCacheC, KV_BF16, KV_E4M3, KV_I8, DT_BF16, DT_F32, EPI_GATE_RESIDUAL, EPI_GELU_TANH, EPI_NONE, GGML_BF16, GGML_F16, GGML_F32,
                    GGML_Q4_0, GGML_Q4_1, GGML_Q4_K, GGML_Q5_0, GGML_Q5_1, GGML_Q5_K, GGML_Q6_K, GGML_Q8_0, check, lib)
 
 # (values, bytes) per GGUF block
@@ -277,6 +277,214 @@ def gguf_inspect(path):
         if line:
             f = line.split("\t")
             out.append((f[0], int(f[1]), tuple(int(x) for x in f[2:])))
+    return out
+
+
+# ---------------------------------------------------------------- text transformers
+
+def _ready(*tensors):
+    """The one device of the tensors (None ones aside), initialised, as an index."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("tensors must be CUDA tensors")
+        d = t.device.index
+        if dev is None:
+            dev = d
+        elif dev != d:
+            raise ValueError(f"tensors on devices {dev} and {d}")
+    if dev not in _inited:
+        with torch.cuda.device(dev):
+            check(lib().mb_init(dev))
+        _inited.add(dev)
+    return dev
+
+
+def _launch(dev, fn, *args):
+    """fn(*args, stream) on device `dev` and its current stream, whichever device is current."""
+    st = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    if dev == torch.cuda.current_device():
+        return check(fn(*args, st))
+    with torch.cuda.device(dev):
+        return check(fn(*args, st))
+
+
+def _heads(x, name, copy=True):
+    """(x, row stride) of a bf16 [rows, heads, D] tensor whose rows are whole and 16-byte aligned; a tensor laid out
+    otherwise is copied, or with copy=False refused."""
+    if x.dim() != 3 or x.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be bf16 [rows, heads, head_dim], got {x.dtype} {tuple(x.shape)}")
+    rows, h, d = x.shape
+    s0, s1, s2 = x.stride()
+    if not (s2 == 1 and (h == 1 or s1 == d) and (rows <= 1 or (s0 >= h * d and s0 % 8 == 0))
+            and x.data_ptr() % 16 == 0):
+        if not copy:
+            raise ValueError(f"{name} must have whole rows, 16-byte aligned (strides {x.stride()})")
+        x = x.clone(memory_format=torch.contiguous_format)
+        s0 = h * d
+    return x, (s0 if rows > 1 else h * d)
+
+
+def _ints(x, name, dim=1):
+    if x.dtype != torch.int32 or x.dim() != dim or (x.numel() and x.stride(-1) != 1 and x.shape[-1] > 1):
+        raise ValueError(f"{name} must be int32 with {dim} dimension(s) and contiguous rows, got {x.dtype} "
+                         f"{tuple(x.shape)}")
+    return x
+
+
+def _table(table, n_seqs):
+    _ints(table, "table", 2)
+    if table.shape[0] != n_seqs:
+        raise ValueError(f"table has {table.shape[0]} rows for {n_seqs} sequences")
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        table = table.contiguous()
+    return table, (table.stride(0) if table.shape[0] > 1 else table.shape[1])
+
+
+def _scale(scale):
+    if scale is None:
+        return 0.0
+    if not scale > 0:
+        raise ValueError(f"scale must be positive, got {scale}")
+    return float(scale)
+
+
+def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None):
+    """Attention of packed prompts with grouped heads: q [Tq, H, D], k / v [Tk, H_kv, D] bf16 -> out [Tq, H, D].
+    Sequence b has query rows [cu_q[b], cu_q[b+1]) and key rows [cu_k[b], cu_k[b+1]) (int32, on the device; cu_k
+    defaults to cu_q); with `causal` its queries are its last positions. A row without keys is 0; rows of out behind
+    the last sequence are not written."""
+    cu_k = cu_q if cu_k is None else cu_k
+    dev = _ready(q, k, v, cu_q, cu_k, out)
+    (q, ldq), (k, ldk), (v, ldv) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    tq, h, d = q.shape
+    if k.shape != v.shape or k.shape[2] != d:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
+    _ints(cu_q, "cu_q"), _ints(cu_k, "cu_k")
+    if cu_q.numel() < 1 or cu_k.numel() != cu_q.numel():
+        raise ValueError("cu_q and cu_k must both have one entry more than there are sequences")
+    if out is None:
+        out = torch.empty((tq, h, d), dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
+    out, ldo = _heads(out, "out", copy=False)
+    _launch(dev, lib().mb_attention_varlen, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, tq, k.shape[0], h,
+            k.shape[1], d, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, int(bool(causal)), _scale(scale),
+            out.data_ptr(), ldo)
+    return out
+
+
+_KV_TYPES = {torch.bfloat16: KV_BF16, torch.int8: KV_I8, torch.float8_e4m3fn: KV_E4M3}
+
+
+class KVCache:
+    """Paged key-value cache of one attention layer: k, v [n_pages, n_kv_heads, page_size, head_dim] in bf16, or in
+    int8 / float8_e4m3fn codes with an f32 scale a row (k_scale, v_scale [n_pages, n_kv_heads, page_size]).
+
+    A sequence's position p is at offset p % page_size of page table[b, p // page_size]; the caller hands out pages.
+    page_size is a power of two from 16 to 256, head_dim 64 or 128."""
+
+    def __init__(self, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.bfloat16, device=None):
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        scales = [None, None] if dtype == torch.bfloat16 else [torch.zeros(shape[:3], device=device) for _ in range(2)]
+        self._hold(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                   *scales)
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale=None, v_scale=None):
+        """A cache over tensors that the caller has; they are used in place."""
+        self = cls.__new__(cls)
+        self._hold(k, v, k_scale, v_scale)
+        return self
+
+    def _hold(self, k, v, k_scale, v_scale):
+        if k.dtype not in _KV_TYPES:
+            raise TypeError(f"unsupported cache dtype {k.dtype}")
+        if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must both be [pages, heads, page, head_dim]")
+        if (k.dtype == torch.bfloat16) != (k_scale is None) or (k_scale is None) != (v_scale is None):
+            raise ValueError("an 8-bit cache has k_scale and v_scale, a bf16 cache has none")
+        for s in (k_scale, v_scale):
+            if s is not None and (s.dtype != torch.float32 or s.shape != k.shape[:3]):
+                raise ValueError(f"scales must be float32 {tuple(k.shape[:3])}")
+        self._tensors = [t for t in (k, v, k_scale, v_scale) if t is not None]
+        if not all(t.is_contiguous() for t in self._tensors):
+            raise ValueError("cache tensors must be contiguous")
+        self.device_index = _ready(*self._tensors)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        self._c = KVCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+                           v_scale.data_ptr() if v_scale is not None else None, self.n_pages, self.page_size,
+                           self.n_kv_heads, self.head_dim, _KV_TYPES[k.dtype])
+
+    def _rows(self, x, name, copy=True):
+        x, ld = _heads(x, name, copy)
+        if x.shape[1:] != (self.n_kv_heads, self.head_dim):
+            raise ValueError(f"{name} is {tuple(x.shape)}, the cache has {self.n_kv_heads} heads of {self.head_dim}")
+        return x, ld
+
+    def write(self, k, v, table, kv_lens, cu=None):
+        """Append rows k, v (bf16 [T, n_kv_heads, head_dim]): sequence b's rows [cu[b], cu[b+1]) become its last
+        positions, kv_lens[b] (int32, the length after the call) at their end. Without cu, row b is sequence b's one
+        new position, and a sequence with kv_lens[b] <= 0 gets none."""
+        dev = _ready(self.k, k, v, table, kv_lens, cu)
+        (k, ldk), (v, ldv) = self._rows(k, "k"), self._rows(v, "v")
+        if k.shape != v.shape:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        n = _ints(kv_lens, "kv_lens").numel()
+        if cu is not None and _ints(cu, "cu").numel() != n + 1:
+            raise ValueError(f"cu has {cu.numel()} entries for {n} sequences")
+        table, ldt = _table(table, n)
+        _launch(dev, lib().mb_kv_write, ctypes.byref(self._c), k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[0],
+                None if cu is None else cu.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), ldt, table.shape[1], n)
+
+    def read(self, table, cu, n_tokens=None, k=None, v=None):
+        """The first cu[b+1] - cu[b] positions of each sequence, packed: k, v bf16 [n_tokens, n_kv_heads, head_dim].
+        n_tokens (default: cu's last entry, which waits for the device) or k and v give the size; rows behind the last
+        sequence are not written."""
+        dev = _ready(self.k, table, cu, k, v)
+        n = _ints(cu, "cu").numel() - 1
+        if n < 0:
+            raise ValueError("cu must have one entry more than there are sequences")
+        if (k is None) != (v is None):
+            raise ValueError("give both k and v or neither")
+        if k is None:
+            n_tokens = int(cu[-1]) if n_tokens is None else int(n_tokens)
+            shape = (n_tokens, self.n_kv_heads, self.head_dim)
+            k, v = (torch.empty(shape, dtype=torch.bfloat16, device=self.k.device) for _ in range(2))
+        (k, ldk), (v, ldv) = self._rows(k, "k", copy=False), self._rows(v, "v", copy=False)
+        if k.shape != v.shape or (n_tokens is not None and n_tokens != k.shape[0]):
+            raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} and n_tokens {n_tokens} do not fit")
+        table, ldt = _table(table, n)
+        _launch(dev, lib().mb_kv_read, ctypes.byref(self._c), cu.data_ptr(), table.data_ptr(), ldt, table.shape[1], n,
+                k.shape[0], k.data_ptr(), ldk, v.data_ptr(), ldv)
+        return k, v
+
+
+def attention_paged(q, cache: KVCache, table, kv_lens, scale=None, out=None):
+    """Attention of one new token of each sequence over its cached positions 0 .. kv_lens[b] - 1: q [B, H, D] bf16 ->
+    out [B, H, D]; a sequence without positions gives 0. Equal calls give equal bits."""
+    dev = _ready(cache.k, q, table, kv_lens, out)
+    q, ldq = _heads(q, "q")
+    n, h, d = q.shape
+    if d != cache.head_dim:
+        raise ValueError(f"q has head_dim {d}, the cache {cache.head_dim}")
+    if _ints(kv_lens, "kv_lens").numel() != n:
+        raise ValueError(f"kv_lens has {kv_lens.numel()} entries for {n} sequences")
+    table, ldt = _table(table, n)
+    if out is None:
+        out = torch.empty((n, h, d), dtype=torch.bfloat16, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
+    out, ldo = _heads(out, "out", copy=False)
+    nbytes = ctypes.c_size_t(0)
+    check(lib().mb_attention_paged_workspace(n, h, cache.n_kv_heads, d, ctypes.byref(nbytes)))
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
+    _launch(dev, lib().mb_attention_paged, q.data_ptr(), ldq, ctypes.byref(cache._c), kv_lens.data_ptr(),
+            table.data_ptr(), ldt, table.shape[1], n, h, _scale(scale), out.data_ptr(), ldo, ws.data_ptr(), nbytes.value)
     return out
 
 
