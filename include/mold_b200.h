@@ -420,7 +420,8 @@ enum { MB_KV_BF16 = 0, MB_KV_I8 = 1, MB_KV_E4M3 = 2 };
 
 /* A paged cache in caller-owned device memory. k, v: [n_pages, n_kv_heads, page_size, head_dim]
  * elements of `dtype`, 16-byte aligned; k_scale, v_scale: f32 [n_pages, n_kv_heads, page_size],
- * 8-byte aligned (NULL for MB_KV_BF16). page_size: a power of two, 16 to 256. A sequence's
+ * 16-byte aligned (NULL for MB_KV_BF16). page_size: a power of two, 16 to 256; fewer than 2^31
+ * (page, head, position) rows. A sequence's
  * position p lies in page table[b][p / page_size] at offset p % page_size (table: device int32,
  * table_width pages of each sequence, rows ld_table apart); entries behind a sequence's last
  * page are not read. */

@@ -1,19 +1,23 @@
 // K14: attention of one new token of each sequence over a paged key-value cache (bf16, or 8-bit codes
 // with a scale a row), split over the cached length and joined.
 //
-// Work is counted in tiles of kWarps * KEYS keys of one unit = (sequence, key head, up to 16 of the
-// query heads that read it). The tiles of all units in a row are cut into equal runs, one for each
-// block of a grid that fills the SMs, so blocks end together however far the lengths lie apart. A
-// block's part of a unit that it does not hold whole goes to the workspace as (max, sum, unnormalised
-// output); k_join adds a unit's parts in the order of the blocks.
+// Work is counted in tiles of kTileKeys keys of one unit = (sequence, key head, up to 16 of the query
+// heads that read it). The tiles of all units in a row are cut into equal runs, one for each block of a
+// grid that fills the SMs, so blocks end together however far the lengths lie apart. A block's part of a
+// unit that it does not hold whole goes to the workspace as (max, sum, unnormalised output); k_join adds
+// a unit's parts in the order of the blocks.
 //
-// Keys and values go from memory straight into the operand registers of the warp matrix products
-// (q k^T: m16n8k16 with the query heads as rows; p v: the same with the keys as depth). Which k index
-// of a product stands for which channel is free as long as both operands agree, so every lane loads 16
-// contiguous bytes of a row and no operand passes through shared memory; values of two keys are paired
-// with a byte permute. 8-bit codes are integers or e4m3 numbers that bf16 holds exactly: the products
-// run on the codes, the key's scale multiplies the score, the value's scale the weight, before the
-// weight's one rounding to bf16. Scores, maximum, sum and output stay in f32.
+// One warp of a block walks the run and keeps a ring of tiles in flight: page numbers, one TMA box of 16
+// keys x 128 bytes after the other (keys, values; 128-byte swizzle), scales and the unit's queries, all
+// landing on the stage's mbarrier. It runs ahead over the borders of units, so a batch of short
+// sequences keeps memory as busy as a long one. Four warps take 16 keys of a tile each: q k^T and p v as
+// m16n8k16 warp products (query heads as rows; at one token a row there is too little arithmetic for
+// more). Which k index of q k^T stands for which channel is free as long as both operands agree, so a
+// lane reads 16 contiguous bytes of a key row. 8-bit codes are integers or e4m3 numbers that bf16 holds
+// exactly: the products run on the codes, the key's scale multiplies the score, the value's scale the
+// weight, before the weight's one rounding to bf16. Scores, maximum, sum and output stay in f32.
+#include <math.h>
+
 #include <string>
 
 #include "common.cuh"
@@ -23,10 +27,11 @@
 namespace mb {
 namespace paged {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kRows = 16;      // query rows of a unit
+constexpr int kWarps = 4;                   // that compute; one more loads
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kRows = 16;                   // query rows of a unit
 constexpr int kBlocksPerSm = 2;
+constexpr int kTileKeys = 16 * kWarps;
 
 struct Part {  // of a unit's work: its first block and how many blocks hold a piece (1: none is joined)
   int first, pieces;
@@ -54,6 +59,12 @@ MB_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+MB_DEV void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
 }
 
 // Two codes as a bf16 pair, exactly. `x` holds them in the low (int8) or high (e4m3) byte of its halves; the other
@@ -84,121 +95,95 @@ MB_DEV uint32_t pair_of_words(uint32_t w0, uint32_t w1, int i) {
                                                : __byte_perm(w0, w1, (i << 4) | ((4 + i) << 12)));
 }
 
-// One warp's keys of a step, in operand registers. KEYS a multiple of 16; lane = 4 g + t.
-//   k: lane (g, t) holds, of key 8 nt + g, the 16 bytes at t of every 64-byte piece of the row.
-//   v: lane (g, t) holds, of keys 16 kg + {2t, 2t + 1, 2t + 8, 2t + 9}, the bytes at g of every eighth.
-template <int CODES, int D, int KEYS>
-struct Tile {
+// A tile's place in shared memory and how its rows are read. A row of 256 bytes lies in two planes of 128-byte
+// lines; shorter rows share or fill a line. The swizzle moves 16-byte pieces inside a line by its number mod 8.
+template <int CODES, int D, bool WIDE>
+struct Shape {
   static constexpr int EB = CODES == MB_KV_BF16 ? 2 : 1;
-  static constexpr int KW = D * EB / 16;              // words of a key row a lane holds
-  static constexpr int VB = D * EB / 8 < 16 ? 8 : 16;  // bytes of a value load
-  static constexpr int VC = D * EB / 8 / VB;          // value loads of a row a lane makes
-  static constexpr int VW = D * EB / 32;              // words of a value row a lane holds
-  uint32_t k[KEYS / 8][KW];
-  uint32_t v[KEYS / 16][4][VW];
-  float2 ks[KEYS / 8], vs[KEYS / 8];
+  static constexpr int ROWB = D * EB;                             // bytes of a row
+  static constexpr int PLANES = ROWB / 128 > 1 ? ROWB / 128 : 1;
+  static constexpr int LINEB = ROWB < 128 ? ROWB : 128;           // bytes of a row in a line
+  static constexpr int GROUPB = 16 * LINEB;                       // 16 keys in a plane
+  static constexpr int PLANEB = kTileKeys * LINEB;
+  static constexpr int KVB = PLANES * PLANEB;
+  static constexpr int SCALEB = CODES == MB_KV_BF16 ? 0 : kTileKeys * 4;
+  static constexpr int STAGEB = 2 * KVB + (2 * SCALEB + 1023) / 1024 * 1024;
+  static constexpr int ROWS = WIDE ? 16 : 8;        // query rows that are kept
+  static constexpr int QB = ROWS * D * 2;
+  static constexpr int QSLOTS = WIDE ? 1 : 2;
+  static constexpr int KS = D / 16;                 // product steps over the channels
+  static constexpr int NR = WIDE ? 4 : 8;           // output column tiles that are merged at a time
+  static constexpr int MERGE_PITCH = NR * 8 + 8;    // floats; 8 (mod 32 banks) from row to row
+  static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
+  static constexpr int kBudget = 113 * 1024 - 1024;  // of a block, two on an SM, 1 KB for alignment
+  static constexpr int kFixed = QSLOTS * QB + MERGEB + 2 * kWarps * kRows * 4 + 1024;
+  static constexpr int STAGES = (kBudget - kFixed) / STAGEB < 8 ? (kBudget - kFixed) / STAGEB : 8;
+  static constexpr size_t kSmem = 1024 + (size_t)STAGES * STAGEB + kFixed;
+  static_assert(STAGES >= 2, "ring too short");
 
-  // rows[i]: cache row of key 16 i of the step, -1 for none; left: keys of the step that exist
-  MB_DEV void load_k(const kv::Cache& c, const int64_t (&rows)[KEYS / 16], int left, int g, int t) {
-#pragma unroll
-    for (int nt = 0; nt < KEYS / 8; nt++) {
-      const int64_t row = rows[nt / 2] + (nt & 1) * 8 + g;
-      const bool ok = rows[nt / 2] >= 0 && nt * 8 + g < left;
-      const uint4* src = (const uint4*)((const uint8_t*)c.k + row * (D * EB)) + t;
-#pragma unroll
-      for (int i = 0; i < KW / 4; i++) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (ok) x = kv::ld_stream(src + 4 * i);
-        k[nt][4 * i] = x.x, k[nt][4 * i + 1] = x.y, k[nt][4 * i + 2] = x.z, k[nt][4 * i + 3] = x.w;
-      }
-      if (CODES != MB_KV_BF16) {
-        const int64_t r2 = rows[nt / 2] + (nt & 1) * 8 + 2 * t;
-        ks[nt] = rows[nt / 2] >= 0 && nt * 8 + 2 * t < left ? *(const float2*)(c.k_scale + r2) : make_float2(0.f, 0.f);
-      }
-    }
+  static MB_DEV uint32_t at(int key, int byte) {  // of a row's byte in K or V, swizzled
+    const uint32_t off = (uint32_t)(key * LINEB + (byte & 127));
+    return (uint32_t)(byte >> 7) * PLANEB + (off ^ ((off >> 3) & 0x70));
   }
-  MB_DEV void load_v(const kv::Cache& c, const int64_t (&rows)[KEYS / 16], int left, int g, int t) {
-#pragma unroll
-    for (int kg = 0; kg < KEYS / 16; kg++) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int key = 2 * t + (j & 1) + (j >> 1) * 8;
-        const bool ok = rows[kg] >= 0 && kg * 16 + key < left;
-        const uint8_t* src = (const uint8_t*)c.v + (rows[kg] + key) * (D * EB) + g * VB;
-#pragma unroll
-        for (int i = 0; i < VC; i++) {
-          if (VB == 16) {
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (ok) x = kv::ld_stream((const uint4*)(src + i * 128));
-            v[kg][j][4 * i] = x.x, v[kg][j][4 * i + 1] = x.y;
-            v[kg][j][4 * i + 2 < VW ? 4 * i + 2 : 0] = x.z, v[kg][j][4 * i + 3 < VW ? 4 * i + 3 : 0] = x.w;
-          } else {
-            uint2 x = make_uint2(0, 0);
-            if (ok) x = kv::ld_stream((const uint2*)src);
-            v[kg][j][0] = x.x, v[kg][j][1] = x.y;
-          }
-        }
-      }
-      if (CODES != MB_KV_BF16) {
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const int key = kg * 16 + u * 8 + 2 * t;
-          const float2 s = rows[kg] >= 0 && key < left ? *(const float2*)(c.v_scale + rows[kg] + u * 8 + 2 * t)
-                                                       : make_float2(0.f, 0.f);
-          vs[kg * 2 + u] = make_float2(s.x, key + 1 < left ? s.y : 0.f);
-        }
-      }
-    }
-  }
-  // operand words (two 16-bit k pairs) of product step s of key row nt
-  MB_DEV void k_operand(int nt, int s, uint32_t& b0, uint32_t& b1) const {
-    if (CODES == MB_KV_BF16) {
-      b0 = k[nt][2 * s], b1 = k[nt][2 * s + 1];
-    } else {
-      b0 = pair_in_word<CODES>(k[nt][s], 0, 1), b1 = pair_in_word<CODES>(k[nt][s], 2, 3);
-    }
-  }
-  // operand words of output column tile n for the 16 keys of group kg
-  MB_DEV void v_operand(int kg, int n, uint32_t& b0, uint32_t& b1) const {
-    if (CODES == MB_KV_BF16) {
-      const int w = n / 2, sel = n & 1 ? 0x7632 : 0x5410;
-      b0 = __byte_perm(v[kg][0][w], v[kg][1][w], sel), b1 = __byte_perm(v[kg][2][w], v[kg][3][w], sel);
-    } else {
-      b0 = pair_of_words<CODES>(v[kg][0][n / 4], v[kg][1][n / 4], n & 3);
-      b1 = pair_of_words<CODES>(v[kg][2][n / 4], v[kg][3][n / 4], n & 3);
-    }
-  }
-  // channel of element (n, column c) of the output
-  static MB_DEV int channel(int n, int c) {
-    return CODES == MB_KV_BF16 ? (n / 8) * 64 + c * 8 + (n & 7) : c * (D / 8) + n;
-  }
-  // first channel of the four that lane t's query operand holds at product step s
+  // first channel of the four that lane t's operands hold at product step s of q k^T
   static MB_DEV int q_channel(int s, int t) {
-    return CODES == MB_KV_BF16 ? (s / 2) * 32 + t * 8 + (s & 1) * 4 : (s / 4) * 64 + t * 16 + (s & 3) * 4;
+    return CODES == MB_KV_BF16 ? (s / 4) * 64 + t * 16 + (s & 3) * 4 : t * (D / 4) + s * 4;
   }
+  // channel of column c of output tile n
+  static MB_DEV int channel(int n, int c) { return CODES == MB_KV_BF16 ? n * 8 + c : c * (D / 8) + n; }
 };
 
-// Run of tiles of block c of n: [first, last)
+// What the loading warp says of a stage.
+struct Desc {
+  int left;         // keys of the tile that exist
+  int groups;       // bit i: its 16 keys from 16 i on are there
+  int q_slot;       // the unit's first tile in this run: where its queries are; else -1
+  int last;         // the unit's last tile in this run
+  int seq, unit;
+  int slot;         // last: workspace slot for the part; -1: the unit is whole
+  int pad;
+};
+
+// Run of tiles of block c of n
 MB_DEV int64_t run_start(int64_t total, int c, int n) { return total * c / n; }
 // The block whose run holds tile t
 MB_DEV int run_owner(int64_t total, int64_t t, int n) { return (int)(((t + 1) * n - 1) / total); }
 
 template <int CODES, int D, bool WIDE>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(const Params p) {
-  constexpr int KEYS = CODES == MB_KV_BF16 ? 16 : 32;
-  constexpr int kTileKeys = kWarps * KEYS;
-  constexpr int ROWS = WIDE ? 16 : 8;
-  constexpr int KS = D / 16;  // product steps over the channels
-  using T = Tile<CODES, D, KEYS>;
-  __shared__ float s_o[kWarps][ROWS][D];
-  __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
-  __shared__ int64_t s_sum[kWarps + 1];
-  __shared__ int64_t s_at;  // tiles before the sequence
-  __shared__ int s_seq;
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+    k_attention_paged(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
+  using S = Shape<CODES, D, WIDE>;
+  constexpr int KS = S::KS, STAGES = S::STAGES;
+  constexpr int RR = WIDE ? 2 : 1;  // rows of a lane: g, g + 8
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* s_q = smem + (size_t)STAGES * S::STAGEB;
+  float* s_merge = (float*)(s_q + S::QSLOTS * S::QB);
+  float* s_m = s_merge + S::MERGEB / 4;  // [kWarps][kRows]
+  float* s_l = s_m + kWarps * kRows;
+  uint64_t* full = (uint64_t*)(s_l + kWarps * kRows);  // [STAGES]
+  uint64_t* empty = full + 8;                          // [STAGES]
+  uint64_t* q_empty = empty + 8;                       // [S::QSLOTS]
+  uint64_t* merge_bar = q_empty + S::QSLOTS;
+  int64_t* s_sum = (int64_t*)(merge_bar + 1);          // [kWarps + 1]
+  int64_t* s_at = s_sum + kWarps + 1;                  // tiles before the run's first sequence
+  Desc* desc = (Desc*)(s_at + 1);                      // [STAGES]
+  int* s_seq = (int*)(desc + 8);
+  volatile int* abort_flag = s_seq + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t cap = (int64_t)p.table_width << p.c.page_log2;
   const int U = p.units_per_seq;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    for (int i = 0; i < S::QSLOTS; i++) mbar_init(&q_empty[i], kWarps);
+    mbar_init(merge_bar, kWarps);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
   auto length = [&](int b) -> int64_t {
     if (b >= p.n_seqs) return 0;
     const int64_t n = __ldg(p.lens + b);
@@ -218,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
     __syncthreads();
     all = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; w++) {
+    for (int w = 0; w <= kWarps; w++) {
       if (w < warp) x += s_sum[w];
       all += s_sum[w];
     }
@@ -244,91 +229,186 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
     if (p.n_seqs > kThreads) incl = scan(base, all); else all = total;
     const int64_t own = tiles_of(length(base + (int)threadIdx.x)) * U;
     const int64_t end = before + incl;
-    if (t0 < end && t0 >= end - own) s_seq = base + threadIdx.x, s_at = end - own;
+    if (t0 < end && t0 >= end - own) *s_seq = base + threadIdx.x, *s_at = end - own;
     before += all;
     if (t0 < before) break;
   }
   __syncthreads();
 
-  int b = s_seq;
-  int64_t at = s_at, tile = t0;
-  while (tile < t1) {
-    int64_t len = length(b);
-    int64_t nt = tiles_of(len);
-    while (tile >= at + nt * U) {  // next sequence that has tiles
-      if (b >= p.n_seqs) return;
-      at += nt * U;
-      len = length(++b);
-      nt = tiles_of(len);
+  if (warp == kWarps) {
+    // ---------------------------------------------------------------- loads
+    if (lane == 0) {
+      tma_prefetch_desc(&tk);
+      tma_prefetch_desc(&tv);
     }
-    const int unit = (int)((tile - at) / nt);
-    const int64_t unit_at = at + unit * nt;
-    const int64_t last = min(t1, unit_at + nt);
-    const int kt0 = (int)(tile - unit_at), kt1 = (int)(last - unit_at);
-    const int hk = unit / p.q_tiles, qt = unit - hk * p.q_tiles;
-    const int rows = min(kRows, p.G - qt * kRows);
-    const int head0 = hk * p.G + qt * kRows;
-
-    // query operand: rows g and g + 8, rows that do not exist 0
-    uint32_t qa[KS][WIDE ? 4 : 2];
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
-      const __nv_bfloat16* src = p.q + (int64_t)b * p.ldq + (int64_t)head0 * D + T::q_channel(s, t);
-      uint2 x = make_uint2(0, 0);
-      if (g < rows) x = *(const uint2*)(src + (int64_t)g * D);
-      qa[s][0] = x.x, qa[s][1] = x.y;
-      if (WIDE) {
-        uint2 y = make_uint2(0, 0);
-        if (g + 8 < rows) y = *(const uint2*)(src + (int64_t)(g + 8) * D);
-        qa[s][WIDE ? 2 : 0] = y.x, qa[s][WIDE ? 3 : 1] = y.y;
-        if (!WIDE) qa[s][0] = x.x, qa[s][1] = x.y;
+    int b = *s_seq, n_seg = 0, it = 0;
+    int64_t at = *s_at, tile = t0;
+    bool ok = true;
+    while (tile < t1 && ok) {
+      int64_t len = length(b);
+      int64_t nt = tiles_of(len);
+      while (tile >= at + nt * U && b < p.n_seqs) {  // next sequence that has tiles
+        at += nt * U;
+        len = length(++b);
+        nt = tiles_of(len);
       }
+      if (b >= p.n_seqs) break;  // lengths that changed under the call
+      const int unit = (int)((tile - at) / nt);
+      const int64_t unit_at = at + unit * nt;
+      const int64_t last = min(t1, unit_at + nt);
+      const int kt0 = (int)(tile - unit_at), kt1 = (int)(last - unit_at);
+      const int hk = unit / p.q_tiles, qt = unit - hk * p.q_tiles;
+      const int rows = min(kRows, p.G - qt * kRows);
+      const bool whole = kt0 == 0 && kt1 == nt;
+      const int32_t* table = p.table + (int64_t)b * p.ld_table;
+      if (kt0 == 0 && lane == 0) {
+        Part part;
+        part.first = c;
+        part.pieces = whole ? 1 : run_owner(total, unit_at + nt - 1, n_blocks) - c + 1;
+        p.parts[(int64_t)b * U + unit] = part;
+      }
+      const int qs = n_seg % S::QSLOTS;
+      for (int kt = kt0; kt < kt1 && ok; kt++, it++) {
+        const int64_t key0 = (int64_t)kt * kTileKeys;
+        const int left = (int)min(len - key0, (int64_t)kTileKeys);
+        int64_t row = -1;
+        if (lane < kWarps && lane * 16 < left)
+          row = kv::row_of(p.c, table, p.table_width, key0 + lane * 16, hk, p.status);
+        const unsigned groups = __ballot_sync(0xffffffffu, row >= 0) & ((1u << kWarps) - 1);
+        const int s = it % STAGES;
+        if (!(ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, kDevTimeoutAttn))) break;
+        if (kt == kt0 &&
+            !(ok = mbar_wait(&q_empty[qs], ((n_seg / S::QSLOTS) & 1) ^ 1, abort_flag, p.status, kDevTimeoutAttn)))
+          break;
+        uint8_t* st = smem + (size_t)s * S::STAGEB;
+        const uint32_t q_bytes = kt == kt0 ? (uint32_t)(rows * D * 2) : 0u;
+        if (lane == 0) {
+          Desc d;
+          d.left = left;
+          d.groups = (int)groups;
+          d.q_slot = kt == kt0 ? qs : -1;
+          d.last = kt == kt1 - 1;
+          d.seq = b;
+          d.unit = unit;
+          d.slot = whole ? -1 : 2 * c + (kt0 == 0 ? 1 : 0);
+          d.pad = 0;
+          desc[s] = d;
+          mbar_expect_tx(&full[s], __popc(groups) * 2u * (16 * S::ROWB + S::SCALEB / kWarps) + q_bytes);
+        }
+        __syncwarp();
+        // lane 8 i + j: copy j of group i (planes of K, planes of V, scales of K, of V)
+        const int gi = lane >> 3, j = lane & 7;
+        const int64_t grow = __shfl_sync(0xffffffffu, row, gi);
+        if (grow >= 0) {
+          if (j < 2 * S::PLANES) {
+            const int plane = j % S::PLANES;
+            const bool is_v = j >= S::PLANES;
+            uint8_t* dst = st + (is_v ? S::KVB : 0) + plane * S::PLANEB + gi * S::GROUPB;
+            // rows shorter than a line lie two to a line of the map
+            tma_load_2d(dst, is_v ? &tv : &tk, &full[s], plane * 128, (int)(grow * S::LINEB / 128));
+          } else if (CODES != MB_KV_BF16 && j >= 4 && j < 6) {
+            bulk_load(st + 2 * S::KVB + (j == 5 ? S::SCALEB : 0) + gi * 64, (j == 5 ? p.c.v_scale : p.c.k_scale) + grow, 64,
+                      &full[s]);
+          }
+        }
+        if (lane == 31 && q_bytes)
+          bulk_load(s_q + qs * S::QB, p.q + (int64_t)b * p.ldq + (int64_t)(hk * p.G + qt * kRows) * D, q_bytes, &full[s]);
+      }
+      n_seg++;
+      tile = last;
     }
-    float o[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const int32_t* table = p.table + (int64_t)b * p.ld_table;
+    // the block's memory must outlive its copies, whatever the other warps do
+    volatile int never = 0;
+    for (int i = it < STAGES ? 0 : it - STAGES; i < it; i++)
+      mbar_wait(&full[i % STAGES], (i / STAGES) & 1, &never, p.status, kDevTimeoutAttn);
+    return;
+  }
 
-    for (int kt = kt0; kt < kt1; kt++) {
-      const int64_t key0 = (int64_t)kt * kTileKeys + warp * KEYS;
-      if (key0 >= len) break;
-      const int left = (int)min(len - key0, (int64_t)KEYS);
-      int64_t rows16[KEYS / 16];
+  // ---------------------------------------------------------------- products
+  uint32_t qa[KS][2 * RR];
+  float o[D / 8][4], m[RR], l[RR];
+  uint32_t merges = 0;
+  const int n_it = (int)(t1 - t0);
+  for (int it = 0; it < n_it; it++) {
+    const int s = it % STAGES;
+    if (!mbar_wait(&full[s], (it / STAGES) & 1, abort_flag, p.status, kDevTimeoutAttn)) break;
+    const Desc d = desc[s];
+    uint8_t* sk = smem + (size_t)s * S::STAGEB;
+    uint8_t* sv = sk + S::KVB;
+    if (d.q_slot >= 0) {
+      const int rows = min(kRows, p.G - (d.unit % p.q_tiles) * kRows);
 #pragma unroll
-      for (int i = 0; i < KEYS / 16; i++)
-        rows16[i] = i * 16 < left ? kv::row_of(p.c, table, p.table_width, key0 + i * 16, hk, p.status) : -1;
-      T x;
-      x.load_k(p.c, rows16, left, g, t);
-      x.load_v(p.c, rows16, left, g, t);
-      float s[KEYS / 8][4];
+      for (int i = 0; i < KS; i++) {
+        const uint8_t* src = s_q + d.q_slot * S::QB + S::q_channel(i, t) * 2;
 #pragma unroll
-      for (int nt8 = 0; nt8 < KEYS / 8; nt8++) {
-        s[nt8][0] = s[nt8][1] = s[nt8][2] = s[nt8][3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < KS; i++) {
-          uint32_t b0, b1;
-          x.k_operand(nt8, i, b0, b1);
-          mma16816(s[nt8], qa[i][0], WIDE ? qa[i][WIDE ? 2 : 0] : 0u, qa[i][1], WIDE ? qa[i][WIDE ? 3 : 1] : 0u, b0, b1);
+        for (int r = 0; r < RR; r++) {
+          uint2 x = make_uint2(0, 0);
+          if (g + 8 * r < rows) x = *(const uint2*)(src + (g + 8 * r) * D * 2);
+          qa[i][2 * r] = x.x, qa[i][2 * r + 1] = x.y;
         }
       }
-      float mx[2] = {-INFINITY, -INFINITY};
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[d.q_slot]);
 #pragma unroll
-      for (int nt8 = 0; nt8 < KEYS / 8; nt8++) {
-        const float f0 = p.scale_log2 * (CODES == MB_KV_BF16 ? 1.f : x.ks[nt8].x);
-        const float f1 = p.scale_log2 * (CODES == MB_KV_BF16 ? 1.f : x.ks[nt8].y);
-        const bool in = rows16[nt8 / 2] >= 0;
-        const bool k0 = in && nt8 * 8 + 2 * t < left, k1 = in && nt8 * 8 + 2 * t + 1 < left;
+      for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-        for (int r = 0; r < (WIDE ? 2 : 1); r++) {
-          s[nt8][2 * r] = k0 ? s[nt8][2 * r] * f0 : -INFINITY;
-          s[nt8][2 * r + 1] = k1 ? s[nt8][2 * r + 1] * f1 : -INFINITY;
-          mx[r] = fmaxf(mx[r], fmaxf(s[nt8][2 * r], s[nt8][2 * r + 1]));
+      for (int r = 0; r < RR; r++) m[r] = -INFINITY, l[r] = 0.f;
+    }
+    const int key0 = warp * 16;
+    if ((d.groups >> warp) & 1) {
+      const int left = d.left - key0;  // of this warp's 16 keys; > 0
+      float sc[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        sc[u][0] = sc[u][1] = sc[u][2] = sc[u][3] = 0.f;
+        const int key = key0 + u * 8 + g;
+        // the lane's bytes of each line: 32 (16 where two rows share a line)
+        constexpr int LB = S::LINEB / 4;
+#pragma unroll
+        for (int pl = 0; pl < S::PLANES; pl++) {
+          uint32_t w[LB / 4];
+#pragma unroll
+          for (int i = 0; i < LB / 16; i++) {
+            const uint4 x = *(const uint4*)(sk + S::at(key, pl * 128 + t * LB + i * 16));
+            w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+          }
+          if (CODES == MB_KV_BF16) {
+#pragma unroll
+            for (int i = 0; i < LB / 8; i++)
+              mma16816(sc[u], qa[pl * 4 + i][0], WIDE ? qa[pl * 4 + i][RR * 2 - 2] : 0u, qa[pl * 4 + i][1],
+                       WIDE ? qa[pl * 4 + i][RR * 2 - 1] : 0u, w[2 * i], w[2 * i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < LB / 4; i++)
+              mma16816(sc[u], qa[i][0], WIDE ? qa[i][RR * 2 - 2] : 0u, qa[i][1], WIDE ? qa[i][RR * 2 - 1] : 0u,
+                       pair_in_word<CODES>(w[i], 0, 1), pair_in_word<CODES>(w[i], 2, 3));
+          }
         }
       }
-      float ref[2], alpha[2];
+      float2 vs[2];
+      float mx[RR], ref[RR], alpha[2] = {1.f, 1.f};
 #pragma unroll
-      for (int r = 0; r < (WIDE ? 2 : 1); r++) {
+      for (int r = 0; r < RR; r++) mx[r] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int k0 = u * 8 + 2 * t;
+        float f0 = p.scale_log2, f1 = p.scale_log2;
+        if (CODES != MB_KV_BF16) {
+          const float2 ks = *(const float2*)(sk + 2 * S::KVB + (key0 + k0) * 4);
+          f0 *= ks.x, f1 *= ks.y;
+          vs[u] = *(const float2*)(sk + 2 * S::KVB + S::SCALEB + (key0 + k0) * 4);
+          if (k0 >= left) vs[u].x = 0.f;  // whatever rows behind the sequence hold
+          if (k0 + 1 >= left) vs[u].y = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < RR; r++) {
+          sc[u][2 * r] = k0 < left ? sc[u][2 * r] * f0 : -INFINITY;
+          sc[u][2 * r + 1] = k0 + 1 < left ? sc[u][2 * r + 1] * f1 : -INFINITY;
+          mx[r] = fmaxf(mx[r], fmaxf(sc[u][2 * r], sc[u][2 * r + 1]));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RR; r++) {
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
         mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
         const float mn = fmaxf(m[r], mx[r]);
@@ -337,7 +417,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
         m[r] = mn;
         l[r] *= alpha[r];
       }
-      if (!WIDE) ref[1] = 0.f, alpha[1] = 1.f;
       if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
         for (int n = 0; n < D / 8; n++) {
@@ -345,75 +424,113 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) k_attention_paged(cons
           if (WIDE) o[n][2] *= alpha[1], o[n][3] *= alpha[1];
         }
       }
+      uint32_t a[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int kg = 0; kg < KEYS / 16; kg++) {
-        uint32_t a[4] = {0u, 0u, 0u, 0u};
+      for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const int nt8 = 2 * kg + u;
+        for (int r = 0; r < RR; r++) {
+          const float p0 = ex2_approx(sc[u][2 * r] - ref[r]), p1 = ex2_approx(sc[u][2 * r + 1] - ref[r]);
+          l[r] += p0 + p1;
+          a[2 * u + r] = CODES == MB_KV_BF16 ? pack_bf16x2(p0, p1) : pack_bf16x2(p0 * vs[u].x, p1 * vs[u].y);
+        }
+      if (CODES == MB_KV_BF16) {
+        // values that do not exist may be NaN: zero their rows first (a tile's partial last group only)
+        if (left < 16) {
+          for (int i = lane; i < (16 - left) * (S::ROWB / 16); i += 32) {
+            const int key = key0 + left + i / (S::ROWB / 16);
+            *(uint4*)(sv + S::at(key, (i % (S::ROWB / 16)) * 16)) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        // one instruction: keys 0-7 and 8-15 of two 8-channel tiles
+        const int key = key0 + (lane & 15);
 #pragma unroll
-          for (int r = 0; r < (WIDE ? 2 : 1); r++) {
-            const float p0 = ex2_approx(s[nt8][2 * r] - ref[r]), p1 = ex2_approx(s[nt8][2 * r + 1] - ref[r]);
-            l[r] += p0 + p1;
-            a[2 * u + r] = CODES == MB_KV_BF16 ? pack_bf16x2(p0, p1) : pack_bf16x2(p0 * x.vs[nt8].x, p1 * x.vs[nt8].y);
+        for (int n = 0; n < D / 8; n += 2) {
+          uint32_t b0, b1, b2, b3;
+          ldmatrix_x4_trans(smem_u32(sv + S::at(key, (n + (lane >> 4)) * 16)), b0, b1, b2, b3);
+          mma16816(o[n], a[0], a[1], a[2], a[3], b0, b1);
+          mma16816(o[n + 1], a[0], a[1], a[2], a[3], b2, b3);
+        }
+      } else {
+        // codes are never NaN, so a weight of 0 silences them
+        constexpr int VB = S::ROWB / 8;  // bytes of a value row a lane reads, of keys 2t, 2t + 1, 2t + 8, 2t + 9
+        uint32_t w[4][VB / 4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint8_t* src = sv + S::at(key0 + 2 * t + (j & 1) + (j >> 1) * 8, (g * VB) & ~15) + ((g * VB) & 15);
+          if (VB == 16) {
+            const uint4 x = *(const uint4*)src;
+            w[j][0] = x.x, w[j][1] = x.y, w[j][VB / 4 - 2] = x.z, w[j][VB / 4 - 1] = x.w;
+          } else {
+            const uint2 x = *(const uint2*)src;
+            w[j][0] = x.x, w[j][1] = x.y;
           }
         }
 #pragma unroll
-        for (int n = 0; n < D / 8; n++) {
-          uint32_t b0, b1;
-          x.v_operand(kg, n, b0, b1);
-          mma16816(o[n], a[0], a[1], a[2], a[3], b0, b1);
-        }
+        for (int n = 0; n < D / 8; n++)
+          mma16816(o[n], a[0], a[1], a[2], a[3], pair_of_words<CODES>(w[0][n / 4], w[1][n / 4], n & 3),
+                   pair_of_words<CODES>(w[2][n / 4], w[3][n / 4], n & 3));
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[s]);
+    if (!d.last) continue;
 
-    // the warps' parts together
+    // the warps' parts together, NR column tiles at a time
+    const int hk = d.unit / p.q_tiles, qt = d.unit - hk * p.q_tiles;
+    const int rows = min(kRows, p.G - qt * kRows), head0 = hk * p.G + qt * kRows;
 #pragma unroll
-    for (int r = 0; r < (WIDE ? 2 : 1); r++) {
+    for (int r = 0; r < RR; r++) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t == 0) s_m[warp][g + 8 * r] = m[r], s_l[warp][g + 8 * r] = l[r];
-#pragma unroll
-      for (int n = 0; n < D / 8; n++) {
-        s_o[warp][g + 8 * r][T::channel(n, 2 * t)] = o[n][2 * r];
-        s_o[warp][g + 8 * r][T::channel(n, 2 * t + 1)] = o[n][2 * r + 1];
-      }
+      if (t == 0) s_m[warp * kRows + g + 8 * r] = m[r], s_l[warp * kRows + g + 8 * r] = l[r];
     }
-    __syncthreads();
-    const bool whole = kt0 == 0 && kt1 == nt;
-    const int64_t slot = 2 * c + (kt0 == 0 ? 1 : 0);
-    constexpr int RP = kThreads / D;  // rows at a time
-    for (int r = threadIdx.x / D; r < rows; r += RP) {
-      const int d = threadIdx.x % D;
-      float top = -INFINITY;
+    bool ok = true;
+    auto meet = [&] {  // of the four warps
+      __syncwarp();
+      if (lane == 0) mbar_arrive(merge_bar);
+      ok = ok && mbar_wait(merge_bar, merges & 1, abort_flag, p.status, kDevTimeoutAttn);
+      merges++;
+    };
 #pragma unroll
-      for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w][r]);
-      const float ref1 = top == -INFINITY ? 0.f : top;
-      float acc = 0.f, sum = 0.f;
+    for (int n0 = 0; n0 < D / 8; n0 += S::NR) {
 #pragma unroll
-      for (int w = 0; w < kWarps; w++) {
-        const float f = ex2_approx(s_m[w][r] - ref1);
-        acc += f * s_o[w][r][d];
-        sum += f * s_l[w][r];
-      }
-      if (whole) {
-        p.out[(int64_t)b * p.ldo + (int64_t)(head0 + r) * D + d] = __float2bfloat16_rn(acc / sum);
-      } else {
-        p.part_o[(slot * kRows + r) * D + d] = acc;
-        if (d == 0) {
-          p.part_ml[slot * 2 * kRows + r] = top;
-          p.part_ml[slot * 2 * kRows + kRows + r] = sum;
+      for (int nl = 0; nl < S::NR; nl++)
+#pragma unroll
+        for (int r = 0; r < RR; r++)
+          *(float2*)(s_merge + (warp * S::ROWS + g + 8 * r) * S::MERGE_PITCH + nl * 8 + 2 * t) =
+              make_float2(o[n0 + nl][2 * r], o[n0 + nl][2 * r + 1]);
+      meet();
+      if (!ok) break;
+      for (int i = threadIdx.x; i < rows * S::NR * 8; i += 32 * kWarps) {
+        const int r = i / (S::NR * 8), nl = i % S::NR, col = (i / S::NR) & 7;
+        const int ch = S::channel(n0 + nl, col);
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w * kRows + r]);
+        const float ref1 = top == -INFINITY ? 0.f : top;
+        float acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+          const float f = ex2_approx(s_m[w * kRows + r] - ref1);
+          acc += f * s_merge[(w * S::ROWS + r) * S::MERGE_PITCH + nl * 8 + col];
+          sum += f * s_l[w * kRows + r];
+        }
+        if (d.slot < 0) {
+          p.out[(int64_t)d.seq * p.ldo + (int64_t)(head0 + r) * D + ch] = __float2bfloat16_rn(acc / sum);
+        } else {
+          p.part_o[((int64_t)d.slot * kRows + r) * D + ch] = acc;
+          if (ch == 0) {
+            p.part_ml[(int64_t)d.slot * 2 * kRows + r] = top;
+            p.part_ml[(int64_t)d.slot * 2 * kRows + kRows + r] = sum;
+          }
         }
       }
+      meet();
+      if (!ok) break;
     }
-    if (kt0 == 0 && threadIdx.x == 0) {
-      Part part;
-      part.first = c;
-      part.pieces = whole ? 1 : run_owner(total, unit_at + nt - 1, n_blocks) - c + 1;
-      p.parts[(int64_t)b * U + unit] = part;
-    }
-    __syncthreads();
-    tile = last;
+    if (!ok) break;
   }
 }
 
@@ -454,13 +571,33 @@ Layout layout(int n_seqs, int H, int H_kv, int D) {
   return a;
 }
 
+template <int CODES, int D, bool WIDE>
+cudaError_t launch_attention(const Params& p, int64_t blocks, cudaStream_t st) {
+  using S = Shape<CODES, D, WIDE>;
+  CUtensorMap tk, tv;
+  // lines of 128 bytes: rows of 256 bytes as two columns of boxes, rows of 64 two to a line
+  const uint64_t inner = S::ROWB < 128 ? 128 : S::ROWB;
+  const uint64_t rows = ((uint64_t)p.c.n_pages * p.c.heads << p.c.page_log2) * S::ROWB / inner;
+  for (int i = 0; i < 2; i++)
+    if (!make_tmap_2d(i ? &tv : &tk, i ? p.c.v : p.c.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, inner, rows, inner, 128,
+                      S::GROUPB / 128, CU_TENSOR_MAP_SWIZZLE_128B))
+      return cudaErrorInvalidValue;
+  static int attr_done[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr_done[dev & 63]) {
+    cudaError_t e = cudaFuncSetAttribute(k_attention_paged<CODES, D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)S::kSmem);
+    if (e != cudaSuccess) return e;
+    attr_done[dev & 63] = 1;
+  }
+  k_attention_paged<CODES, D, WIDE><<<(unsigned)blocks, kThreads, S::kSmem, st>>>(tk, tv, p);
+  return cudaGetLastError();
+}
+
 template <int CODES, int D>
 cudaError_t launch(const Params& p, int64_t blocks, int64_t units, cudaStream_t st) {
-  if (p.G > 8)
-    k_attention_paged<CODES, D, true><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-  else
-    k_attention_paged<CODES, D, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = p.G > 8 ? launch_attention<CODES, D, true>(p, blocks, st) : launch_attention<CODES, D, false>(p, blocks, st);
   if (e != cudaSuccess) return e;
   k_join<D><<<dim3((unsigned)units, (unsigned)(p.G < kRows ? p.G : kRows)), D, 0, st>>>(p);
   return cudaGetLastError();

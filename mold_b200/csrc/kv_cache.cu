@@ -197,12 +197,14 @@ mb_status check_kv_cache(const mb_kv_cache* c) {
            "page_size must be a power of two from 16 to 256");
   MB_CHECK(c->n_kv_heads > 0 && c->n_kv_heads <= 65535 && c->n_pages > 0 && c->n_pages < (1LL << 31), MB_ERR_INVALID,
            "cache sizes must be positive, n_pages below 2^31 and n_kv_heads below 65536");
+  MB_CHECK(c->n_pages < (1LL << 31) / ((int64_t)c->n_kv_heads * c->page_size), MB_ERR_INVALID,
+           "n_pages * n_kv_heads * page_size must be below 2^31");
   MB_CHECK(c->k && c->v, MB_ERR_INVALID, "cache k or v is NULL");
   MB_CHECK(((uintptr_t)c->k & 15) == 0 && ((uintptr_t)c->v & 15) == 0, MB_ERR_INVALID,
            "cache k and v must be 16-byte aligned");
   if (c->dtype != MB_KV_BF16)
-    MB_CHECK(c->k_scale && c->v_scale && ((uintptr_t)c->k_scale & 7) == 0 && ((uintptr_t)c->v_scale & 7) == 0,
-             MB_ERR_INVALID, "an 8-bit cache needs 8-byte aligned k_scale and v_scale");
+    MB_CHECK(c->k_scale && c->v_scale && ((uintptr_t)c->k_scale & 15) == 0 && ((uintptr_t)c->v_scale & 15) == 0,
+             MB_ERR_INVALID, "an 8-bit cache needs 16-byte aligned k_scale and v_scale");
   return MB_OK;
 }
 
