@@ -11,11 +11,17 @@
 // keys x 128 bytes after the other (keys, values; 128-byte swizzle), scales and the unit's queries, all
 // landing on the stage's mbarrier. It runs ahead over the borders of units, so a batch of short
 // sequences keeps memory as busy as a long one. Four warps take 16 keys of a tile each: q k^T and p v as
-// m16n8k16 warp products (query heads as rows; at one token a row there is too little arithmetic for
-// more). Which k index of q k^T stands for which channel is free as long as both operands agree, so a
-// lane reads 16 contiguous bytes of a key row. 8-bit codes are integers or e4m3 numbers that bf16 holds
-// exactly: the products run on the codes, the key's scale multiplies the score, the value's scale the
-// weight, before the weight's one rounding to bf16. Scores, maximum, sum and output stay in f32.
+// warp products (query heads as rows; at one token a row there is too little arithmetic for more). Which
+// k index of q k^T stands for which channel is free as long as both operands agree, so a lane reads 16
+// contiguous bytes of a key row. Scores, maximum, sum and output stay in f32.
+//
+// 8-bit caches: the products run on the codes, the key's scale multiplies the score, the value's scale
+// the weight. q k^T needs no conversion of codes: the queries become two 8-bit digits (int8: q = s (256 h
+// + l), off by at most 2^-16 of the row's largest magnitude; e4m3: q = 2^e (h + l), off by at most 2^-17
+// of it, exact for what is not far smaller), which fill the 16 rows of one product where up to 8 heads
+// share a key head. Values become f16, which holds every code exactly, and the weights are rounded to
+// f16 as p * (value scale / largest value scale so far) * 2^15, relative to 2^-11 down to 2^-29 of the
+// largest. Converting both operands to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
 #include <math.h>
 
 #include <string>
@@ -67,32 +73,76 @@ MB_DEV void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_
                : "memory");
 }
 
-// Two codes as a bf16 pair, exactly. `x` holds them in the low (int8) or high (e4m3) byte of its halves; the other
-// bytes may hold anything.
-//   int8: the low seven bits under the exponent of 128 give 128 + (c mod 128); the sign bit makes 256 of the 128
-//   that is taken off.
-//   e4m3: exponent and mantissa bits moved to bf16's places give c * 2^-120, subnormal codes included.
+MB_DEV void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Products of 8-bit codes, 32 channels at a time; c holds int32 (int8) or f32 (e4m3).
 template <int CODES>
-MB_DEV uint32_t codes_bf16x2(uint32_t x) {
-  __nv_bfloat162 r;
+MB_DEV void mma16832(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (CODES == MB_KV_I8)
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 keys x 32 channels of codes, transposed: r[2 i + j] holds, for channel 16 i + 8 j + g, keys 4t .. 4t + 3.
+MB_DEV void ldmatrix_b8_x2_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// The four codes of a word as two f16 pairs, exactly. int8: byte c + 128 under the exponent of 1024 is 1152 + c.
+template <int CODES>
+MB_DEV void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (CODES == MB_KV_I8) {
-    const uint32_t a = (x & 0x007f007fu) | 0x43004300u, b = (x & 0x00800080u) | 0x43004300u;
-    r = __hsub2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*(const __half2*)&a, off), y = __hsub2(*(const __half2*)&b, off);
+    lo = *(const uint32_t*)&x, hi = *(const uint32_t*)&y;
   } else {
-    const uint32_t a = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u), b = 0x7b807b80u;
-    r = __hmul2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+    asm("{\n .reg .b16 x, y;\n mov.b32 {x, y}, %2;\n cvt.rn.f16x2.e4m3x2 %0, x;\n cvt.rn.f16x2.e4m3x2 %1, y;\n}\n"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   }
-  return *(uint32_t*)&r;
 }
-// Bytes i and j of w (8-bit codes of neighbouring channels), or byte i of two words, as a bf16 pair.
+
+// Four neighbouring channels of a query row (bf16 pairs x, y) as a word of high and one of low digits; `f` brings the
+// row's largest magnitude to 32639 (int8) or below 256 (e4m3, a power of two).
 template <int CODES>
-MB_DEV uint32_t pair_in_word(uint32_t w, int i, int j) {
-  return codes_bf16x2<CODES>(CODES == MB_KV_I8 ? __byte_perm(w, 0, i | (j << 8)) : __byte_perm(w, 0, (i << 4) | (j << 12)));
-}
-template <int CODES>
-MB_DEV uint32_t pair_of_words(uint32_t w0, uint32_t w1, int i) {
-  return codes_bf16x2<CODES>(CODES == MB_KV_I8 ? __byte_perm(w0, w1, i | ((4 + i) << 8))
-                                               : __byte_perm(w0, w1, (i << 4) | ((4 + i) << 12)));
+MB_DEV void query_digits(uint2 x, float f, uint32_t& h, uint32_t& l) {
+  const float q[4] = {bf16_lo(x.x) * f, bf16_hi(x.x) * f, bf16_lo(x.y) * f, bf16_hi(x.y) * f};
+  if (CODES == MB_KV_I8) {
+    h = l = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int v = __float2int_rn(q[i]), hi = (v + 128) >> 8;  // low digit in [-128, 127]
+      h |= ((uint32_t)hi & 255u) << (8 * i);
+      l |= ((uint32_t)v & 255u) << (8 * i);
+    }
+  } else {
+    uint16_t c[2], d[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c[i]) : "f"(q[2 * i + 1]), "f"(q[2 * i]));
+      uint32_t back;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(c[i]));
+      const float2 b = __half22float2(*(const __half2*)&back);
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d[i]) : "f"(q[2 * i + 1] - b.y), "f"(q[2 * i] - b.x));
+    }
+    h = (uint32_t)c[0] | ((uint32_t)c[1] << 16);
+    l = (uint32_t)d[0] | ((uint32_t)d[1] << 16);
+  }
 }
 
 // A tile's place in shared memory and how its rows are read. A row of 256 bytes lies in two planes of 128-byte
@@ -111,12 +161,12 @@ struct Shape {
   static constexpr int ROWS = WIDE ? 16 : 8;        // query rows that are kept
   static constexpr int QB = ROWS * D * 2;
   static constexpr int QSLOTS = WIDE ? 1 : 2;
-  static constexpr int KS = D / 16;                 // product steps over the channels
+  static constexpr int KS = D / 16;                 // product steps over the channels (of 16, bf16)
   static constexpr int NR = WIDE ? 4 : 8;           // output column tiles that are merged at a time
   static constexpr int MERGE_PITCH = NR * 8 + 8;    // floats; 8 (mod 32 banks) from row to row
   static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
   static constexpr int kBudget = 113 * 1024 - 1024;  // of a block, two on an SM, 1 KB for alignment
-  static constexpr int kFixed = QSLOTS * QB + MERGEB + 2 * kWarps * kRows * 4 + 1024;
+  static constexpr int kFixed = QSLOTS * QB + MERGEB + 2 * kWarps * kRows * 4 + 1024;  // and barriers, descriptors
   static constexpr int STAGES = (kBudget - kFixed) / STAGEB < 8 ? (kBudget - kFixed) / STAGEB : 8;
   static constexpr size_t kSmem = 1024 + (size_t)STAGES * STAGEB + kFixed;
   static_assert(STAGES >= 2, "ring too short");
@@ -125,12 +175,13 @@ struct Shape {
     const uint32_t off = (uint32_t)(key * LINEB + (byte & 127));
     return (uint32_t)(byte >> 7) * PLANEB + (off ^ ((off >> 3) & 0x70));
   }
-  // first channel of the four that lane t's operands hold at product step s of q k^T
-  static MB_DEV int q_channel(int s, int t) {
-    return CODES == MB_KV_BF16 ? (s / 4) * 64 + t * 16 + (s & 3) * 4 : t * (D / 4) + s * 4;
+  // first channel of the four that lane t's operands hold at product step s of q k^T (bf16)
+  static MB_DEV int q_channel(int s, int t) { return (s / 4) * 64 + t * 16 + (s & 3) * 4; }
+  // The key of a warp's 16 that is column j of score tile u. Values of 8-bit types come as keys 4t .. 4t + 3 a lane,
+  // so the weights have to as well.
+  static MB_DEV int key_of(int u, int j) {
+    return CODES == MB_KV_BF16 ? u * 8 + j : (j >> 1) * 4 + u * 2 + (j & 1);
   }
-  // channel of column c of output tile n
-  static MB_DEV int channel(int n, int c) { return CODES == MB_KV_BF16 ? n * 8 + c : c * (D / 8) + n; }
 };
 
 // What the loading warp says of a stage.
@@ -168,7 +219,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   int64_t* s_sum = (int64_t*)(merge_bar + 1);          // [kWarps + 1]
   int64_t* s_at = s_sum + kWarps + 1;                  // tiles before the run's first sequence
   Desc* desc = (Desc*)(s_at + 1);                      // [STAGES]
-  int* s_seq = (int*)(desc + 8);
+  float* s_v = (float*)(desc + 8);                     // [kWarps]
+  int* s_seq = (int*)(s_v + kWarps);
   volatile int* abort_flag = s_seq + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -325,8 +377,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   }
 
   // ---------------------------------------------------------------- products
-  uint32_t qa[KS][2 * RR];
+  // Query operand. bf16: qa[step][2 r + half]. 8-bit: digits[r][0 high, 1 low][word of 4 channels], and what brings the
+  // row's scores back to size.
+  constexpr bool B16 = CODES == MB_KV_BF16;
+  constexpr int QW = D / 16;  // words of four channels that a lane holds of a row
+  uint32_t qa[B16 ? KS : 1][2 * RR], digits[RR][2][B16 ? 1 : QW];
+  float q_size[RR];
   float o[D / 8][4], m[RR], l[RR];
+  float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and 2^15 over it
   uint32_t merges = 0;
   const int n_it = (int)(t1 - t0);
   for (int it = 0; it < n_it; it++) {
@@ -338,13 +396,45 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     if (d.q_slot >= 0) {
       const int rows = min(kRows, p.G - (d.unit % p.q_tiles) * kRows);
 #pragma unroll
-      for (int i = 0; i < KS; i++) {
-        const uint8_t* src = s_q + d.q_slot * S::QB + S::q_channel(i, t) * 2;
+      for (int r = 0; r < RR; r++) {
+        const bool have = g + 8 * r < rows;
+        const uint8_t* src = s_q + d.q_slot * S::QB + (g + 8 * r) * D * 2;
+        if (B16) {
+          q_size[r] = p.scale_log2;
 #pragma unroll
-        for (int r = 0; r < RR; r++) {
-          uint2 x = make_uint2(0, 0);
-          if (g + 8 * r < rows) x = *(const uint2*)(src + (g + 8 * r) * D * 2);
-          qa[i][2 * r] = x.x, qa[i][2 * r + 1] = x.y;
+          for (int i = 0; i < KS; i++) {
+            uint2 x = make_uint2(0, 0);
+            if (have) x = *(const uint2*)(src + S::q_channel(i, t) * 2);
+            qa[B16 ? i : 0][2 * r] = x.x, qa[B16 ? i : 0][2 * r + 1] = x.y;
+          }
+        } else {
+          uint2 x[QW];
+          uint32_t top = 0;  // largest magnitude's bits: non-negative floats order like integers, NaN last
+#pragma unroll
+          for (int i = 0; i < QW; i++) {
+            x[i] = make_uint2(0, 0);
+            if (have) x[i] = *(const uint2*)(src + (t * (D / 4) + i * 4) * 2);
+            top = max(top, max((x[i].x << 16) & 0x7fff0000u, (x[i].y << 16) & 0x7fff0000u));
+            top = max(top, max(x[i].x & 0x7fff0000u, x[i].y & 0x7fff0000u));
+          }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          float f, back;
+          if (CODES == MB_KV_I8) {
+            // below 2^-100 the row counts as 0
+            const bool some = top >= 0x0d800000u;
+            f = some ? 32639.f / __uint_as_float(top) : 0.f;
+            back = some ? __uint_as_float(top) / 32639.f : 0.f;
+          } else {
+            const int e = max((int)(top >> 23), 8);
+            f = __uint_as_float((uint32_t)(261 - e) << 23);   // 2^(134 - e)
+            back = __uint_as_float((uint32_t)(e > 8 ? e - 7 : 1) << 23);
+          }
+          if (top >= 0x7f800000u) f = 0.f, back = __uint_as_float(0x7fc00000u);  // NaN or infinity in the row
+          q_size[r] = back * p.scale_log2;
+#pragma unroll
+          for (int i = 0; i < QW; i++)
+            query_digits<CODES>(x[i], f, digits[r][0][B16 ? 0 : i], digits[r][1][B16 ? 0 : i]);
         }
       }
       __syncwarp();
@@ -353,17 +443,19 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
       for (int r = 0; r < RR; r++) m[r] = -INFINITY, l[r] = 0.f;
+      v_ref = v_inv = 0.f;
     }
     const int key0 = warp * 16;
     if ((d.groups >> warp) & 1) {
       const int left = d.left - key0;  // of this warp's 16 keys; > 0
-      float sc[2][4];
+      float sc[2][2 * RR];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        sc[u][0] = sc[u][1] = sc[u][2] = sc[u][3] = 0.f;
-        const int key = key0 + u * 8 + g;
+        const int key = key0 + S::key_of(u, g);
         // the lane's bytes of each line: 32 (16 where two rows share a line)
         constexpr int LB = S::LINEB / 4;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t ch[4] = {0u, 0u, 0u, 0u}, cl[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int pl = 0; pl < S::PLANES; pl++) {
           uint32_t w[LB / 4];
@@ -372,16 +464,33 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
             const uint4 x = *(const uint4*)(sk + S::at(key, pl * 128 + t * LB + i * 16));
             w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
           }
-          if (CODES == MB_KV_BF16) {
+          if (B16) {
 #pragma unroll
-            for (int i = 0; i < LB / 8; i++)
-              mma16816(sc[u], qa[pl * 4 + i][0], WIDE ? qa[pl * 4 + i][RR * 2 - 2] : 0u, qa[pl * 4 + i][1],
-                       WIDE ? qa[pl * 4 + i][RR * 2 - 1] : 0u, w[2 * i], w[2 * i + 1]);
+            for (int i = 0; i < LB / 8; i++) {
+              const uint32_t* a = qa[B16 ? pl * 4 + i : 0];
+              mma16816(acc, a[0], WIDE ? a[2 * RR - 2] : 0u, a[1], WIDE ? a[2 * RR - 1] : 0u, w[2 * i], w[2 * i + 1]);
+            }
           } else {
 #pragma unroll
-            for (int i = 0; i < LB / 4; i++)
-              mma16816(sc[u], qa[i][0], WIDE ? qa[i][RR * 2 - 2] : 0u, qa[i][1], WIDE ? qa[i][RR * 2 - 1] : 0u,
-                       pair_in_word<CODES>(w[i], 0, 1), pair_in_word<CODES>(w[i], 2, 3));
+            for (int i = 0; i < LB / 8; i++) {
+              const int x = B16 ? 0 : 2 * i, y = B16 ? 0 : 2 * i + 1;
+              if (WIDE) {
+                mma16832<CODES>(ch, digits[0][0][x], digits[RR - 1][0][x], digits[0][0][y], digits[RR - 1][0][y], w[2 * i], w[2 * i + 1]);
+                mma16832<CODES>(cl, digits[0][1][x], digits[RR - 1][1][x], digits[0][1][y], digits[RR - 1][1][y], w[2 * i], w[2 * i + 1]);
+              } else {  // high digits as rows 0-7, low ones as rows 8-15
+                mma16832<CODES>(ch, digits[0][0][x], digits[0][1][x], digits[0][0][y], digits[0][1][y], w[2 * i], w[2 * i + 1]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * RR; e++) {
+          if (B16) {
+            sc[u][e] = acc[e];
+          } else {
+            const uint32_t hi = ch[e], lo = WIDE ? cl[e] : ch[e + 2 < 4 ? e + 2 : e];
+            // int8: 256 h + l is below 2^30
+            sc[u][e] = CODES == MB_KV_I8 ? (float)((int)hi * 256 + (int)lo) : __uint_as_float(hi) + __uint_as_float(lo);
           }
         }
       }
@@ -391,20 +500,31 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       for (int r = 0; r < RR; r++) mx[r] = -INFINITY;
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const int k0 = u * 8 + 2 * t;
-        float f0 = p.scale_log2, f1 = p.scale_log2;
-        if (CODES != MB_KV_BF16) {
+        const int k0 = S::key_of(u, 2 * t);  // and the next one
+        float f0 = 1.f, f1 = 1.f;
+        if (!B16) {
           const float2 ks = *(const float2*)(sk + 2 * S::KVB + (key0 + k0) * 4);
-          f0 *= ks.x, f1 *= ks.y;
+          f0 = ks.x, f1 = ks.y;
           vs[u] = *(const float2*)(sk + 2 * S::KVB + S::SCALEB + (key0 + k0) * 4);
           if (k0 >= left) vs[u].x = 0.f;  // whatever rows behind the sequence hold
           if (k0 + 1 >= left) vs[u].y = 0.f;
         }
 #pragma unroll
         for (int r = 0; r < RR; r++) {
-          sc[u][2 * r] = k0 < left ? sc[u][2 * r] * f0 : -INFINITY;
-          sc[u][2 * r + 1] = k0 + 1 < left ? sc[u][2 * r + 1] * f1 : -INFINITY;
+          sc[u][2 * r] = k0 < left ? sc[u][2 * r] * (f0 * q_size[r]) : -INFINITY;
+          sc[u][2 * r + 1] = k0 + 1 < left ? sc[u][2 * r + 1] * (f1 * q_size[r]) : -INFINITY;
           mx[r] = fmaxf(mx[r], fmaxf(sc[u][2 * r], sc[u][2 * r + 1]));
+        }
+      }
+      float shrink = 1.f;
+      if (!B16) {
+        float vm = fmaxf(fmaxf(vs[0].x, vs[0].y), fmaxf(vs[1].x, vs[1].y));
+        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
+        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
+        if (vm > v_ref) {  // the same in all lanes
+          shrink = v_ref / vm;
+          v_ref = vm;
+          v_inv = 32768.f / vm;
         }
       }
 #pragma unroll
@@ -416,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         alpha[r] = ex2_approx(m[r] - ref[r]);
         m[r] = mn;
         l[r] *= alpha[r];
+        alpha[r] *= shrink;
       }
       if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
@@ -431,9 +552,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         for (int r = 0; r < RR; r++) {
           const float p0 = ex2_approx(sc[u][2 * r] - ref[r]), p1 = ex2_approx(sc[u][2 * r + 1] - ref[r]);
           l[r] += p0 + p1;
-          a[2 * u + r] = CODES == MB_KV_BF16 ? pack_bf16x2(p0, p1) : pack_bf16x2(p0 * vs[u].x, p1 * vs[u].y);
+          if (B16) {
+            a[2 * u + r] = pack_bf16x2(p0, p1);
+          } else {
+            const __half2 h = __floats2half2_rn(p0 * (vs[u].x * v_inv), p1 * (vs[u].y * v_inv));
+            a[2 * u + r] = *(const uint32_t*)&h;
+          }
         }
-      if (CODES == MB_KV_BF16) {
+      if (B16) {
         // values that do not exist may be NaN: zero their rows first (a tile's partial last group only)
         if (left < 16) {
           for (int i = lane; i < (16 - left) * (S::ROWB / 16); i += 32) {
@@ -453,24 +579,21 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
           mma16816(o[n + 1], a[0], a[1], a[2], a[3], b2, b3);
         }
       } else {
-        // codes are never NaN, so a weight of 0 silences them
-        constexpr int VB = S::ROWB / 8;  // bytes of a value row a lane reads, of keys 2t, 2t + 1, 2t + 8, 2t + 9
-        uint32_t w[4][VB / 4];
+        // a weight of 0 silences codes of rows that do not exist, but for e4m3's NaN: those become 0
+        const int key = key0 + (lane & 15);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint8_t* src = sv + S::at(key0 + 2 * t + (j & 1) + (j >> 1) * 8, (g * VB) & ~15) + ((g * VB) & 15);
-          if (VB == 16) {
-            const uint4 x = *(const uint4*)src;
-            w[j][0] = x.x, w[j][1] = x.y, w[j][VB / 4 - 2] = x.z, w[j][VB / 4 - 1] = x.w;
-          } else {
-            const uint2 x = *(const uint2*)src;
-            w[j][0] = x.x, w[j][1] = x.y;
+        for (int n = 0; n < D / 8; n += 4) {
+          uint32_t w[4];
+          ldmatrix_b8_x2_trans(smem_u32(sv + S::at(key, (n / 2 + (lane >> 4)) * 16)), w);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint32_t b0, b1;
+            if (CODES == MB_KV_E4M3 && left < 16)
+              w[i] &= 4 * t >= left ? 0u : left - 4 * t >= 4 ? 0xffffffffu : (1u << (8 * (left - 4 * t))) - 1u;
+            codes_f16<CODES>(w[i], b0, b1);
+            mma16816_f16(o[n + i], a[0], a[1], a[2], a[3], b0, b1);
           }
         }
-#pragma unroll
-        for (int n = 0; n < D / 8; n++)
-          mma16816(o[n], a[0], a[1], a[2], a[3], pair_of_words<CODES>(w[0][n / 4], w[1][n / 4], n & 3),
-                   pair_of_words<CODES>(w[2][n / 4], w[3][n / 4], n & 3));
       }
     }
     __syncwarp();
@@ -486,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       if (t == 0) s_m[warp * kRows + g + 8 * r] = m[r], s_l[warp * kRows + g + 8 * r] = l[r];
     }
+    if (lane == 0) s_v[warp] = B16 ? 1.f : v_ref * 0x1p-15f;
     bool ok = true;
     auto meet = [&] {  // of the four warps
       __syncwarp();
@@ -504,8 +628,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       meet();
       if (!ok) break;
       for (int i = threadIdx.x; i < rows * S::NR * 8; i += 32 * kWarps) {
-        const int r = i / (S::NR * 8), nl = i % S::NR, col = (i / S::NR) & 7;
-        const int ch = S::channel(n0 + nl, col);
+        const int r = i / (S::NR * 8), nl = (i >> 3) % S::NR, col = i & 7;
+        const int ch = (n0 + nl) * 8 + col;
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w * kRows + r]);
@@ -514,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
           const float f = ex2_approx(s_m[w * kRows + r] - ref1);
-          acc += f * s_merge[(w * S::ROWS + r) * S::MERGE_PITCH + nl * 8 + col];
+          acc += f * s_v[w] * s_merge[(w * S::ROWS + r) * S::MERGE_PITCH + nl * 8 + col];
           sum += f * s_l[w * kRows + r];
         }
         if (d.slot < 0) {
