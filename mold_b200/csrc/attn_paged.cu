@@ -162,8 +162,8 @@ struct Shape {
   static constexpr int QB = ROWS * D * 2;
   static constexpr int QSLOTS = WIDE ? 1 : 2;
   static constexpr int KS = D / 16;                 // product steps over the channels (of 16, bf16)
-  static constexpr int NR = WIDE ? 4 : 8;           // output column tiles that are merged at a time
-  static constexpr int MERGE_PITCH = NR * 8 + 8;    // floats; 8 (mod 32 banks) from row to row
+  static constexpr int NR = WIDE ? 2 : 4;           // 16-channel output tiles that are merged at a time
+  static constexpr int MERGE_PITCH = NR * 16 + 4;   // floats; rows 2t begin 8 banks apart
   static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
   static constexpr int kBudget = 113 * 1024 - 1024;  // of a block, two on an SM, 1 KB for alignment
   static constexpr int kFixed = QSLOTS * QB + MERGEB + 2 * kWarps * kRows * 4 + 1024;  // and barriers, descriptors
@@ -320,13 +320,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         p.parts[(int64_t)b * U + unit] = part;
       }
       const int qs = n_seg % S::QSLOTS;
+      int64_t row32 = -1;  // cache row of 16-key group lane of the next 32
       for (int kt = kt0; kt < kt1 && ok; kt++, it++) {
         const int64_t key0 = (int64_t)kt * kTileKeys;
         const int left = (int)min(len - key0, (int64_t)kTileKeys);
-        int64_t row = -1;
-        if (lane < kWarps && lane * 16 < left)
-          row = kv::row_of(p.c, table, p.table_width, key0 + lane * 16, hk, p.status);
-        const unsigned groups = __ballot_sync(0xffffffffu, row >= 0) & ((1u << kWarps) - 1);
+        const int ahead = (kt - kt0) % (32 / kWarps) * kWarps;  // this tile's first group among them
+        if (ahead == 0) {
+          const int64_t k32 = key0 + lane * 16;
+          row32 = kt + lane / kWarps < kt1 && k32 < len ? kv::row_of(p.c, table, p.table_width, k32, hk, p.status) : -1;
+        }
+        const unsigned groups = (__ballot_sync(0xffffffffu, row32 >= 0) >> ahead) & ((1u << kWarps) - 1);
         const int s = it % STAGES;
         if (!(ok = mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, kDevTimeoutAttn))) break;
         if (kt == kt0 &&
@@ -350,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
         __syncwarp();
         // lane 8 i + j: copy j of group i (planes of K, planes of V, scales of K, of V)
         const int gi = lane >> 3, j = lane & 7;
-        const int64_t grow = __shfl_sync(0xffffffffu, row, gi);
+        const int64_t grow = __shfl_sync(0xffffffffu, row32, ahead + gi);
         if (grow >= 0) {
           if (j < 2 * S::PLANES) {
             const int plane = j % S::PLANES;
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   constexpr int QW = D / 16;  // words of four channels that a lane holds of a row
   uint32_t qa[B16 ? KS : 1][2 * RR], digits[RR][2][B16 ? 1 : QW];
   float q_size[RR];
-  float o[D / 8][4], m[RR], l[RR];
+  float o[RR][D / 16][4], m[RR], l[RR];  // o: channels 16 i + g (0, 1) and + 8 (2, 3), rows 8 r + 2t and + 1
   float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and 2^15 over it
   uint32_t merges = 0;
   const int n_it = (int)(t1 - t0);
@@ -440,9 +443,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[d.q_slot]);
 #pragma unroll
-      for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+      for (int r = 0; r < RR; r++) {
 #pragma unroll
-      for (int r = 0; r < RR; r++) m[r] = -INFINITY, l[r] = 0.f;
+        for (int i = 0; i < D / 16; i++) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.f;
+        m[r] = -INFINITY, l[r] = 0.f;
+      }
       v_ref = v_inv = 0.f;
     }
     const int key0 = warp * 16;
@@ -540,12 +545,15 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       }
       if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-        for (int n = 0; n < D / 8; n++) {
-          o[n][0] *= alpha[0], o[n][1] *= alpha[0];
-          if (WIDE) o[n][2] *= alpha[1], o[n][3] *= alpha[1];
+        for (int r = 0; r < RR; r++) {
+          const float a0 = __shfl_sync(0xffffffffu, alpha[r], 8 * t), a1 = __shfl_sync(0xffffffffu, alpha[r], 8 * t + 4);
+#pragma unroll
+          for (int i = 0; i < D / 16; i++) o[r][i][0] *= a0, o[r][i][1] *= a1, o[r][i][2] *= a0, o[r][i][3] *= a1;
         }
       }
-      uint32_t a[4] = {0u, 0u, 0u, 0u};
+      // The scores' accumulator layout (row g, keys 2t) is that of a B operand with keys as depth: the output is formed
+      // transposed, values as A (16 channels), weights as B (8 rows), and no row of a product is idle.
+      uint32_t w8[RR][2];
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -553,10 +561,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
           const float p0 = ex2_approx(sc[u][2 * r] - ref[r]), p1 = ex2_approx(sc[u][2 * r + 1] - ref[r]);
           l[r] += p0 + p1;
           if (B16) {
-            a[2 * u + r] = pack_bf16x2(p0, p1);
+            w8[r][u] = pack_bf16x2(p0, p1);
           } else {
             const __half2 h = __floats2half2_rn(p0 * (vs[u].x * v_inv), p1 * (vs[u].y * v_inv));
-            a[2 * u + r] = *(const uint32_t*)&h;
+            w8[r][u] = *(const uint32_t*)&h;
           }
         }
       if (B16) {
@@ -569,29 +577,34 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        // one instruction: keys 0-7 and 8-15 of two 8-channel tiles
-        const int key = key0 + (lane & 15);
+        // one instruction: channels 16 i and 16 i + 8 of keys 0-7, then of keys 8-15
+        const int key = key0 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-        for (int n = 0; n < D / 8; n += 2) {
-          uint32_t b0, b1, b2, b3;
-          ldmatrix_x4_trans(smem_u32(sv + S::at(key, (n + (lane >> 4)) * 16)), b0, b1, b2, b3);
-          mma16816(o[n], a[0], a[1], a[2], a[3], b0, b1);
-          mma16816(o[n + 1], a[0], a[1], a[2], a[3], b2, b3);
+        for (int i = 0; i < D / 16; i++) {
+          uint32_t a0, a1, a2, a3;
+          ldmatrix_x4_trans(smem_u32(sv + S::at(key, (2 * i + ((lane >> 3) & 1)) * 16)), a0, a1, a2, a3);
+#pragma unroll
+          for (int r = 0; r < RR; r++) mma16816(o[r][i], a0, a1, a2, a3, w8[r][0], w8[r][1]);
         }
       } else {
         // a weight of 0 silences codes of rows that do not exist, but for e4m3's NaN: those become 0
         const int key = key0 + (lane & 15);
 #pragma unroll
-        for (int n = 0; n < D / 8; n += 4) {
+        for (int i = 0; i < D / 16; i += 2) {
           uint32_t w[4];
-          ldmatrix_b8_x2_trans(smem_u32(sv + S::at(key, (n / 2 + (lane >> 4)) * 16)), w);
+          ldmatrix_b8_x2_trans(smem_u32(sv + S::at(key, (i + (lane >> 4)) * 16)), w);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            uint32_t b0, b1;
-            if (CODES == MB_KV_E4M3 && left < 16)
-              w[i] &= 4 * t >= left ? 0u : left - 4 * t >= 4 ? 0xffffffffu : (1u << (8 * (left - 4 * t))) - 1u;
-            codes_f16<CODES>(w[i], b0, b1);
-            mma16816_f16(o[n + i], a[0], a[1], a[2], a[3], b0, b1);
+          for (int j = 0; j < 2; j++) {
+            uint32_t a[4];  // {channels g, g + 8} x {keys 4t, 4t + 1; 4t + 2, 4t + 3}
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              uint32_t x = w[2 * j + e];
+              if (CODES == MB_KV_E4M3 && left < 16)
+                x &= 4 * t >= left ? 0u : left - 4 * t >= 4 ? 0xffffffffu : (1u << (8 * (left - 4 * t))) - 1u;
+              codes_f16<CODES>(x, a[e], a[2 + e]);
+            }
+#pragma unroll
+            for (int r = 0; r < RR; r++) mma16816_f16(o[r][i + j], a[0], a[1], a[2], a[3], w8[r][0], w8[r][1]);
           }
         }
       }
@@ -618,18 +631,18 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
       merges++;
     };
 #pragma unroll
-    for (int n0 = 0; n0 < D / 8; n0 += S::NR) {
+    for (int i0 = 0; i0 < D / 16; i0 += S::NR) {
 #pragma unroll
-      for (int nl = 0; nl < S::NR; nl++)
+      for (int i = 0; i < S::NR; i++)
 #pragma unroll
         for (int r = 0; r < RR; r++)
-          *(float2*)(s_merge + (warp * S::ROWS + g + 8 * r) * S::MERGE_PITCH + nl * 8 + 2 * t) =
-              make_float2(o[n0 + nl][2 * r], o[n0 + nl][2 * r + 1]);
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            s_merge[(warp * S::ROWS + 8 * r + 2 * t + (e & 1)) * S::MERGE_PITCH + i * 16 + g + (e >> 1) * 8] = o[r][i0 + i][e];
       meet();
       if (!ok) break;
-      for (int i = threadIdx.x; i < rows * S::NR * 8; i += 32 * kWarps) {
-        const int r = i / (S::NR * 8), nl = (i >> 3) % S::NR, col = i & 7;
-        const int ch = (n0 + nl) * 8 + col;
+      for (int i = threadIdx.x; i < rows * S::NR * 16; i += 32 * kWarps) {
+        const int r = i / (S::NR * 16), col = i % (S::NR * 16), ch = i0 * 16 + col;
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w * kRows + r]);
@@ -638,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
           const float f = ex2_approx(s_m[w * kRows + r] - ref1);
-          acc += f * s_v[w] * s_merge[(w * S::ROWS + r) * S::MERGE_PITCH + nl * 8 + col];
+          acc += f * s_v[w] * s_merge[(w * S::ROWS + r) * S::MERGE_PITCH + col];
           sum += f * s_l[w * kRows + r];
         }
         if (d.slot < 0) {
