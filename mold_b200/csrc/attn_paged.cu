@@ -36,7 +36,7 @@ namespace paged {
 constexpr int kWarps = 4;                   // that compute; one more loads
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kRows = 16;                   // query rows of a unit
-constexpr int kBlocksPerSm = 2;
+constexpr int kMaxBlocksPerSm = 3;
 constexpr int kTileKeys = 16 * kWarps;
 
 struct Part {  // of a unit's work: its first block and how many blocks hold a piece (1: none is joined)
@@ -165,7 +165,8 @@ struct Shape {
   static constexpr int NR = WIDE ? 2 : 4;           // 16-channel output tiles that are merged at a time
   static constexpr int MERGE_PITCH = NR * 16 + 4;   // floats; rows 2t begin 8 banks apart
   static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
-  static constexpr int kBudget = 113 * 1024 - 1024;  // of a block, two on an SM, 1 KB for alignment
+  static constexpr int BLOCKS = CODES == MB_KV_BF16 || WIDE ? 2 : 3;  // on an SM
+  static constexpr int kBudget = (228 / BLOCKS - 2) * 1024;  // of a block: 1 KB is the system's, 1 KB for alignment
   static constexpr int kFixed = QSLOTS * QB + MERGEB + 2 * kWarps * kRows * 4 + 1024;  // and barriers, descriptors
   static constexpr int STAGES = (kBudget - kFixed) / STAGEB < 8 ? (kBudget - kFixed) / STAGEB : 8;
   static constexpr size_t kSmem = 1024 + (size_t)STAGES * STAGEB + kFixed;
@@ -201,7 +202,7 @@ MB_DEV int64_t run_start(int64_t total, int c, int n) { return total * c / n; }
 MB_DEV int run_owner(int64_t total, int64_t t, int n) { return (int)(((t + 1) * n - 1) / total); }
 
 template <int CODES, int D, bool WIDE>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+__global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     k_attention_paged(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
   using S = Shape<CODES, D, WIDE>;
   constexpr int KS = S::KS, STAGES = S::STAGES;
@@ -701,7 +702,7 @@ struct Layout {
 Layout layout(int n_seqs, int H, int H_kv, int D) {
   Layout a;
   a.units = (int64_t)n_seqs * H_kv * ((H / H_kv + kRows - 1) / kRows);
-  a.blocks = (int64_t)num_sms() * kBlocksPerSm;
+  a.blocks = (int64_t)num_sms() * kMaxBlocksPerSm;
   a.ml = ((size_t)a.units * sizeof(Part) + 255) / 256 * 256;
   a.o = a.ml + (size_t)a.blocks * 2 * 2 * kRows * sizeof(float);
   a.bytes = a.o + (size_t)a.blocks * 2 * kRows * D * sizeof(float);
@@ -709,7 +710,7 @@ Layout layout(int n_seqs, int H, int H_kv, int D) {
 }
 
 template <int CODES, int D, bool WIDE>
-cudaError_t launch_attention(const Params& p, int64_t blocks, cudaStream_t st) {
+cudaError_t launch_attention(const Params& p, cudaStream_t st) {
   using S = Shape<CODES, D, WIDE>;
   CUtensorMap tk, tv;
   // lines of 128 bytes: rows of 256 bytes as two columns of boxes, rows of 64 two to a line
@@ -728,13 +729,13 @@ cudaError_t launch_attention(const Params& p, int64_t blocks, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     attr_done[dev & 63] = 1;
   }
-  k_attention_paged<CODES, D, WIDE><<<(unsigned)blocks, kThreads, S::kSmem, st>>>(tk, tv, p);
+  k_attention_paged<CODES, D, WIDE><<<(unsigned)(num_sms() * S::BLOCKS), kThreads, S::kSmem, st>>>(tk, tv, p);
   return cudaGetLastError();
 }
 
 template <int CODES, int D>
-cudaError_t launch(const Params& p, int64_t blocks, int64_t units, cudaStream_t st) {
-  cudaError_t e = p.G > 8 ? launch_attention<CODES, D, true>(p, blocks, st) : launch_attention<CODES, D, false>(p, blocks, st);
+cudaError_t launch(const Params& p, int64_t units, cudaStream_t st) {
+  cudaError_t e = p.G > 8 ? launch_attention<CODES, D, true>(p, st) : launch_attention<CODES, D, false>(p, st);
   if (e != cudaSuccess) return e;
   k_join<D><<<dim3((unsigned)units, (unsigned)(p.G < kRows ? p.G : kRows)), D, 0, st>>>(p);
   return cudaGetLastError();
@@ -806,13 +807,13 @@ mb_status mb_attention_paged(const void* q, int64_t ldq, const mb_kv_cache* cach
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (D == 64)
-    e = cache->dtype == MB_KV_BF16 ? paged::launch<MB_KV_BF16, 64>(p, a.blocks, a.units, st)
-        : cache->dtype == MB_KV_I8 ? paged::launch<MB_KV_I8, 64>(p, a.blocks, a.units, st)
-                                   : paged::launch<MB_KV_E4M3, 64>(p, a.blocks, a.units, st);
+    e = cache->dtype == MB_KV_BF16 ? paged::launch<MB_KV_BF16, 64>(p, a.units, st)
+        : cache->dtype == MB_KV_I8 ? paged::launch<MB_KV_I8, 64>(p, a.units, st)
+                                   : paged::launch<MB_KV_E4M3, 64>(p, a.units, st);
   else
-    e = cache->dtype == MB_KV_BF16 ? paged::launch<MB_KV_BF16, 128>(p, a.blocks, a.units, st)
-        : cache->dtype == MB_KV_I8 ? paged::launch<MB_KV_I8, 128>(p, a.blocks, a.units, st)
-                                   : paged::launch<MB_KV_E4M3, 128>(p, a.blocks, a.units, st);
+    e = cache->dtype == MB_KV_BF16 ? paged::launch<MB_KV_BF16, 128>(p, a.units, st)
+        : cache->dtype == MB_KV_I8 ? paged::launch<MB_KV_I8, 128>(p, a.units, st)
+                                   : paged::launch<MB_KV_E4M3, 128>(p, a.units, st);
   MB_CUDA(e);
   return MB_OK;
 }
