@@ -20,8 +20,8 @@
 // + l), off by at most 2^-16 of the row's largest magnitude; e4m3: q = 2^e (h + l), off by at most 2^-17
 // of it, exact for what is not far smaller), which fill the 16 rows of one product where up to 8 heads
 // share a key head. Values become f16, which holds every code exactly, and the weights are rounded to
-// f16 as p * (value scale / largest value scale so far) * 2^15, relative to 2^-11 down to 2^-29 of the
-// largest. Converting both operands to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
+// f16 as p * (value scale / largest value scale so far) * 2^11, relative to 2^-11 down to 2^-25 of the
+// largest and to 2^-36 of it below. Converting both operands to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
 #include <math.h>
 
 #include <string>
@@ -38,6 +38,8 @@ constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kRows = 16;                   // query rows of a unit
 constexpr int kMaxBlocksPerSm = 3;
 constexpr int kTileKeys = 16 * kWarps;
+constexpr float kSlack = 4.f;               // log2 of how far a weight may pass 1
+constexpr float kWeightOne = 2048.f;        // f16 form of a weight of 1 with the largest value scale: 2^15 at most
 
 struct Part {  // of a unit's work: its first block and how many blocks hold a piece (1: none is joined)
   int first, pieces;
@@ -61,7 +63,7 @@ struct Params {
 };
 
 MB_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -69,12 +71,11 @@ MB_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
 MB_DEV void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 
 MB_DEV void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -83,12 +84,12 @@ MB_DEV void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
 template <int CODES>
 MB_DEV void mma16832(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (CODES == MB_KV_I8)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -97,8 +98,7 @@ MB_DEV void mma16832(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, ui
 MB_DEV void ldmatrix_b8_x2_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 
 // The four codes of a word as two f16 pairs, exactly. int8: byte c + 128 under the exponent of 1024 is 1152 + c.
@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
   uint32_t qa[B16 ? KS : 1][2 * RR], digits[RR][2][B16 ? 1 : QW];
   float q_size[RR];
   float o[RR][D / 16][4], m[RR], l[RR];  // o: channels 16 i + g (0, 1) and + 8 (2, 3), rows 8 r + 2t and + 1
-  float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and 2^15 over it
+  float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and kWeightOne over it
   uint32_t merges = 0;
   const int n_it = (int)(t1 - t0);
   for (int it = 0; it < n_it; it++) {
@@ -454,6 +454,16 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     const int key0 = warp * 16;
     if ((d.groups >> warp) & 1) {
       const int left = d.left - key0;  // of this warp's 16 keys; > 0
+      // 8-bit values are read ahead of the scores, whose latency hides theirs; where 16 rows leave no registers for
+      // them, when their turn comes
+      uint32_t vw[B16 ? 1 : D / 32][4];
+      auto load_v = [&](int i) {
+        ldmatrix_b8_x2_trans(smem_u32(sv + S::at(key0 + (lane & 15), (2 * i + (lane >> 4)) * 16)), vw[B16 ? 0 : i]);
+      };
+      if (!B16 && !WIDE) {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) load_v(i);
+      }
       float sc[2][2 * RR];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
@@ -501,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
         }
       }
       float2 vs[2];
-      float mx[RR], ref[RR], alpha[2] = {1.f, 1.f};
+      float mx[RR], ref[RR];
 #pragma unroll
       for (int r = 0; r < RR; r++) mx[r] = -INFINITY;
 #pragma unroll
@@ -522,36 +532,40 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
           mx[r] = fmaxf(mx[r], fmaxf(sc[u][2 * r], sc[u][2 * r + 1]));
         }
       }
-      float shrink = 1.f;
-      if (!B16) {
-        float vm = fmaxf(fmaxf(vs[0].x, vs[0].y), fmaxf(vs[1].x, vs[1].y));
-        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
-        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
-        if (vm > v_ref) {  // the same in all lanes
-          shrink = v_ref / vm;
-          v_ref = vm;
-          v_inv = 32768.f / vm;
-        }
-      }
+      // The reference points move (and the output with them) only when a score passes its row's by more than 2^kSlack,
+      // or a value scale the largest so far.
+      float vm = 0.f;
+      if (!B16) vm = fmaxf(fmaxf(vs[0].x, vs[0].y), fmaxf(vs[1].x, vs[1].y));
+      bool move = vm > v_ref;
 #pragma unroll
-      for (int r = 0; r < RR; r++) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        const float mn = fmaxf(m[r], mx[r]);
-        ref[r] = mn == -INFINITY ? 0.f : mn;  // nothing but -inf so far: weights 0
-        alpha[r] = ex2_approx(m[r] - ref[r]);
-        m[r] = mn;
-        l[r] *= alpha[r];
-        alpha[r] *= shrink;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+      for (int r = 0; r < RR; r++) move |= mx[r] > m[r] + kSlack;
+      if (__any_sync(0xffffffffu, move)) {
+        float shrink = 1.f;
+        if (!B16) {
+          vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
+          vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
+          if (vm > v_ref) {  // the same in all lanes
+            shrink = v_ref / vm;
+            v_ref = vm;
+            v_inv = kWeightOne / vm;
+          }
+        }
 #pragma unroll
         for (int r = 0; r < RR; r++) {
-          const float a0 = __shfl_sync(0xffffffffu, alpha[r], 8 * t), a1 = __shfl_sync(0xffffffffu, alpha[r], 8 * t + 4);
+          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+          const float mn = mx[r] > m[r] + kSlack ? mx[r] : m[r];
+          float alpha = mn == -INFINITY ? 1.f : ex2_approx(m[r] - mn);
+          m[r] = mn;
+          l[r] *= alpha;
+          alpha *= shrink;
+          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
 #pragma unroll
           for (int i = 0; i < D / 16; i++) o[r][i][0] *= a0, o[r][i][1] *= a1, o[r][i][2] *= a0, o[r][i][3] *= a1;
         }
       }
+#pragma unroll
+      for (int r = 0; r < RR; r++) ref[r] = m[r] == -INFINITY ? 0.f : m[r];  // nothing but -inf so far: weights 0
       // The scores' accumulator layout (row g, keys 2t) is that of a B operand with keys as depth: the output is formed
       // transposed, values as A (16 channels), weights as B (8 rows), and no row of a product is idle.
       uint32_t w8[RR][2];
@@ -589,17 +603,15 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
         }
       } else {
         // a weight of 0 silences codes of rows that do not exist, but for e4m3's NaN: those become 0
-        const int key = key0 + (lane & 15);
 #pragma unroll
         for (int i = 0; i < D / 16; i += 2) {
-          uint32_t w[4];
-          ldmatrix_b8_x2_trans(smem_u32(sv + S::at(key, (i + (lane >> 4)) * 16)), w);
+          if (WIDE) load_v(i / 2);
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             uint32_t a[4];  // {channels g, g + 8} x {keys 4t, 4t + 1; 4t + 2, 4t + 3}
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              uint32_t x = w[2 * j + e];
+              uint32_t x = vw[B16 ? 0 : i / 2][2 * j + e];
               if (CODES == MB_KV_E4M3 && left < 16)
                 x &= 4 * t >= left ? 0u : left - 4 * t >= 4 ? 0xffffffffu : (1u << (8 * (left - 4 * t))) - 1u;
               codes_f16<CODES>(x, a[e], a[2 + e]);
@@ -623,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       if (t == 0) s_m[warp * kRows + g + 8 * r] = m[r], s_l[warp * kRows + g + 8 * r] = l[r];
     }
-    if (lane == 0) s_v[warp] = B16 ? 1.f : v_ref * 0x1p-15f;
+    if (lane == 0) s_v[warp] = B16 ? 1.f : v_ref / kWeightOne;
     bool ok = true;
     auto meet = [&] {  // of the four warps
       __syncwarp();

@@ -316,7 +316,8 @@ def test_bad_pages_are_reported_and_not_touched(cuda):
     assert mb.device_status() == _lib.DEV_BAD_PAGE
     for b, left in ((0, list(range(16)) + list(range(32, 40))), (1, list(range(32)))):
         kk, vv = U.cached64(cache, pages, b, 40)
-        ref, tol = U.attention64(q[b:b + 1], kk[left], vv[left], torch.ones((1, len(left)), dtype=torch.bool, device="cuda"))
+        keep = torch.ones((1, len(left)), dtype=torch.bool, device="cuda")
+        ref, tol = U.attention64(q[b:b + 1], kk[left], vv[left], keep, half_weights=True)
         close(out[b:b + 1], ref, tol)
 
 
@@ -339,7 +340,8 @@ def filled(dtype, lengths, page, Hkv, D, seed, width=None):
 def check_paged(q, cache, pages, lengths, out, scale=None):
     for b, n in enumerate(lengths):
         k, v = U.cached64(cache, pages, b, n)
-        ref, tol = U.attention64(q[b:b + 1], k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"), scale)
+        ref, tol = U.attention64(q[b:b + 1], k, v, torch.ones((1, n), dtype=torch.bool, device="cuda"), scale,
+                                 half_weights=cache.k.dtype != torch.bfloat16)
         close(out[b:b + 1], ref, tol)
 
 
@@ -368,7 +370,7 @@ def test_paged_splits(cuda, dtype, lengths):
     for b in some:
         k, v = U.cached64(cache, pages, b, lengths[b])
         keep = torch.ones((1, lengths[b]), dtype=torch.bool, device="cuda")
-        close(out[b:b + 1], *U.attention64(q[b:b + 1], k, v, keep))
+        close(out[b:b + 1], *U.attention64(q[b:b + 1], k, v, keep, half_weights=dtype != torch.bfloat16))
 
 
 def test_paged_layouts_scale_and_padding(cuda):

@@ -13,7 +13,7 @@ def offsets(lengths, device="cuda"):
     return torch.tensor(at, dtype=torch.int32, device=device)
 
 
-def attention64(q, k, v, keep, scale=None):
+def attention64(q, k, v, keep, scale=None, half_weights=False):
     """q [m, H, D], k / v [n, H_kv, D], keep [m, n] (bool) -> (out, tolerance), both f64 [m, H, D].
 
     Tolerance of the kernels' result against out, element by element, with A = sum_j w_j |v_j|:
@@ -21,6 +21,11 @@ def attention64(q, k, v, keep, scale=None):
       2^-8 A            each weight's rounding to bf16 before the product with v
       2 d A, d = D 2^-23 max_j scale sum |q k_j|   the f32 accumulation of the scores (D additions, each off by at most
                         one step, in numerator and denominator)
+      n 2^-36 max |v|   with half_weights (8-bit caches): the weights are f16 numbers, 2^11 standing for a weight of 1
+                        on the row with the largest value scale. Below f16's 2^-14 they are off by up to half its last
+                        step, 2^-25, which is 2^-36 of that row's largest value; the n weights' sum is at least 1, the
+                        weight of the reference score. Above, 2^-11 of the weight is within the 2^-8 A, and so are the
+                        query's digits: off by 2^-17 max |q| a channel, times sum |k| scale, far below 2^-9
       2^-11 A           exponentials (polynomial 7.5e-5 = 2^-13.7, MUFU 2^-22) in numerator and denominator, f32 sums
     """
     m, H, D = q.shape
@@ -40,6 +45,8 @@ def attention64(q, k, v, keep, scale=None):
     w = w / torch.where(total > 0, total, torch.ones_like(total))
     out, a = w @ v, w @ v.abs()
     tol = 2.0 ** -8 * out.abs() + (2.0 ** -8 + 2.0 ** -11 + 2 * off) * a
+    if half_weights:
+        tol = tol + n * 2.0 ** -36 * v.abs().amax()
     return out.transpose(0, 1), tol.transpose(0, 1)
 
 
