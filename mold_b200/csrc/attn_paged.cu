@@ -15,13 +15,20 @@
 // k index of q k^T stands for which channel is free as long as both operands agree, so a lane reads 16
 // contiguous bytes of a key row. Scores, maximum, sum and output stay in f32.
 //
+// Both products are formed transposed: keys (16) are the rows of K q^T and channels those of V^T p^T, with
+// 8 query heads as columns, so that no row of a product is idle where few heads share a key head. A
+// register transposition (movmatrix) takes the weights from one to the other.
+//
 // 8-bit caches: the products run on the codes, the key's scale multiplies the score, the value's scale
-// the weight. q k^T needs no conversion of codes: the queries become two 8-bit digits (int8: q = s (256 h
-// + l), off by at most 2^-16 of the row's largest magnitude; e4m3: q = 2^e (h + l), off by at most 2^-17
-// of it, exact for what is not far smaller), which fill the 16 rows of one product where up to 8 heads
-// share a key head. Values become f16, which holds every code exactly, and the weights are rounded to
-// f16 as p * (value scale / largest value scale so far) * 2^11, relative to 2^-11 down to 2^-25 of the
-// largest and to 2^-36 of it below. Converting both operands to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
+// the weight.
+//   int8 scores need no conversion of codes: a query becomes s (256 h + l) with int8 digits h and l, off by
+//   at most 2^-16 of its row's largest magnitude, and the integer sums are exact.
+//   e4m3 scores: codes to f16, which holds every code, with the query row times a power of two in f16 (off
+//   by at most 2^-25 of the row's largest magnitude). The 8-bit float product is no help here: it measured
+//   as many instructions as the conversion.
+//   Values become f16, and the weights are rounded to f16 as p * (value scale / largest value scale so far)
+//   * 2^11, relative to 2^-11 down to 2^-25 of the largest and to 2^-36 of it below.
+// Converting codes to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
 #include <math.h>
 
 #include <string>
@@ -80,19 +87,17 @@ MB_DEV void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Products of 8-bit codes, 32 channels at a time; c holds int32 (int8) or f32 (e4m3).
-template <int CODES>
-MB_DEV void mma16832(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if (CODES == MB_KV_I8)
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// 32 channels of int8 codes; exact.
+MB_DEV void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of 16-bit elements held as row g, columns 2t and 2t + 1 a lane.
+MB_DEV uint32_t movmatrix(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 // 16 keys x 32 channels of codes, transposed: r[2 i + j] holds, for channel 16 i + 8 j + g, keys 4t .. 4t + 3.
 MB_DEV void ldmatrix_b8_x2_trans(uint32_t addr, uint32_t (&r)[4]) {
@@ -118,31 +123,20 @@ MB_DEV void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
 }
 
 // Four neighbouring channels of a query row (bf16 pairs x, y) as a word of high and one of low digits; `f` brings the
-// row's largest magnitude to 32639 (int8) or below 256 (e4m3, a power of two).
-template <int CODES>
+// row's largest magnitude to 32639.
 MB_DEV void query_digits(uint2 x, float f, uint32_t& h, uint32_t& l) {
   const float q[4] = {bf16_lo(x.x) * f, bf16_hi(x.x) * f, bf16_lo(x.y) * f, bf16_hi(x.y) * f};
-  if (CODES == MB_KV_I8) {
-    h = l = 0;
+  h = l = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int v = __float2int_rn(q[i]), hi = (v + 128) >> 8;  // low digit in [-128, 127]
-      h |= ((uint32_t)hi & 255u) << (8 * i);
-      l |= ((uint32_t)v & 255u) << (8 * i);
-    }
-  } else {
-    uint16_t c[2], d[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c[i]) : "f"(q[2 * i + 1]), "f"(q[2 * i]));
-      uint32_t back;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(c[i]));
-      const float2 b = __half22float2(*(const __half2*)&back);
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d[i]) : "f"(q[2 * i + 1] - b.y), "f"(q[2 * i] - b.x));
-    }
-    h = (uint32_t)c[0] | ((uint32_t)c[1] << 16);
-    l = (uint32_t)d[0] | ((uint32_t)d[1] << 16);
+  for (int i = 0; i < 4; i++) {
+    const int v = __float2int_rn(q[i]), hi = (v + 128) >> 8;  // low digit in [-128, 127]
+    h |= ((uint32_t)hi & 255u) << (8 * i);
+    l |= ((uint32_t)v & 255u) << (8 * i);
   }
+}
+MB_DEV uint32_t scaled_f16x2(uint32_t x, float f) {
+  const __half2 h = __floats2half2_rn(bf16_lo(x) * f, bf16_hi(x) * f);
+  return *(const uint32_t*)&h;
 }
 
 // A tile's place in shared memory and how its rows are read. A row of 256 bytes lies in two planes of 128-byte
@@ -161,7 +155,7 @@ struct Shape {
   static constexpr int ROWS = WIDE ? 16 : 8;        // query rows that are kept
   static constexpr int QB = ROWS * D * 2;
   static constexpr int QSLOTS = WIDE ? 1 : 2;
-  static constexpr int KS = D / 16;                 // product steps over the channels (of 16, bf16)
+  static constexpr int QW = D / 16;                 // four-channel groups of a row that a lane holds
   static constexpr int NR = WIDE ? 2 : 4;           // 16-channel output tiles that are merged at a time
   static constexpr int MERGE_PITCH = NR * 16 + 4;   // floats; rows 2t begin 8 banks apart
   static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
@@ -176,9 +170,11 @@ struct Shape {
     const uint32_t off = (uint32_t)(key * LINEB + (byte & 127));
     return (uint32_t)(byte >> 7) * PLANEB + (off ^ ((off >> 3) & 0x70));
   }
-  // first channel of the four that lane t's operands hold at product step s of q k^T (bf16)
-  static MB_DEV int q_channel(int s, int t) { return (s / 4) * 64 + t * 16 + (s & 3) * 4; }
-  // The key of a warp's 16 that is column j of score tile u. Values of 8-bit types come as keys 4t .. 4t + 3 a lane,
+  // first channel of group w of the four-channel groups that lane t holds of a row
+  static MB_DEV int q_channel(int w, int t) {
+    return CODES == MB_KV_BF16 ? (w / 4) * 64 + t * 16 + (w & 3) * 4 : t * (D / 4) + w * 4;
+  }
+  // The key of a warp's 16 that is row 8 u + j of the scores. Values of 8-bit types come as keys 4t .. 4t + 3 a lane,
   // so the weights have to as well.
   static MB_DEV int key_of(int u, int j) {
     return CODES == MB_KV_BF16 ? u * 8 + j : (j >> 1) * 4 + u * 2 + (j & 1);
@@ -205,8 +201,8 @@ template <int CODES, int D, bool WIDE>
 __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     k_attention_paged(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
   using S = Shape<CODES, D, WIDE>;
-  constexpr int KS = S::KS, STAGES = S::STAGES;
-  constexpr int RR = WIDE ? 2 : 1;  // rows of a lane: g, g + 8
+  constexpr int QW = S::QW, STAGES = S::STAGES;
+  constexpr int RR = WIDE ? 2 : 1;  // eights of query rows
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = smem + (size_t)STAGES * S::STAGEB;
@@ -381,13 +377,13 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
   }
 
   // ---------------------------------------------------------------- products
-  // Query operand. bf16: qa[step][2 r + half]. 8-bit: digits[r][0 high, 1 low][word of 4 channels], and what brings the
-  // row's scores back to size.
-  constexpr bool B16 = CODES == MB_KV_BF16;
-  constexpr int QW = D / 16;  // words of four channels that a lane holds of a row
-  uint32_t qa[B16 ? KS : 1][2 * RR], digits[RR][2][B16 ? 1 : QW];
-  float q_size[RR];
-  float o[RR][D / 16][4], m[RR], l[RR];  // o: channels 16 i + g (0, 1) and + 8 (2, 3), rows 8 r + 2t and + 1
+  // Query operand of row 8 r + g, by four-channel groups: two pairs (bf16; f16 for e4m3), or a high and a low digit word
+  // (int8); and what brings the scores of rows 8 r + 2t and + 1 back to size, times log2(e).
+  constexpr bool B16 = CODES == MB_KV_BF16, I8 = CODES == MB_KV_I8;
+  uint32_t qa[RR][QW][2];
+  float q_size[RR][2];
+  // o: channels 16 i + g (0, 1) and + 8 (2, 3) of rows 8 r + 2t and + 1; m, l: of these rows
+  float o[RR][D / 16][4], m[RR][2], l[RR][2];
   float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and kWeightOne over it
   uint32_t merges = 0;
   const int n_it = (int)(t1 - t0);
@@ -403,52 +399,52 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
       for (int r = 0; r < RR; r++) {
         const bool have = g + 8 * r < rows;
         const uint8_t* src = s_q + d.q_slot * S::QB + (g + 8 * r) * D * 2;
-        if (B16) {
-          q_size[r] = p.scale_log2;
+        uint32_t top = 0;  // largest magnitude's bits: non-negative floats order like integers, NaN last
 #pragma unroll
-          for (int i = 0; i < KS; i++) {
-            uint2 x = make_uint2(0, 0);
-            if (have) x = *(const uint2*)(src + S::q_channel(i, t) * 2);
-            qa[B16 ? i : 0][2 * r] = x.x, qa[B16 ? i : 0][2 * r + 1] = x.y;
+        for (int i = 0; i < QW; i++) {
+          uint2 x = make_uint2(0, 0);
+          if (have) x = *(const uint2*)(src + S::q_channel(i, t) * 2);
+          qa[r][i][0] = x.x, qa[r][i][1] = x.y;
+          if (!B16) {
+            top = max(top, max((x.x << 16) & 0x7fff0000u, (x.y << 16) & 0x7fff0000u));
+            top = max(top, max(x.x & 0x7fff0000u, x.y & 0x7fff0000u));
           }
-        } else {
-          uint2 x[QW];
-          uint32_t top = 0;  // largest magnitude's bits: non-negative floats order like integers, NaN last
-#pragma unroll
-          for (int i = 0; i < QW; i++) {
-            x[i] = make_uint2(0, 0);
-            if (have) x[i] = *(const uint2*)(src + (t * (D / 4) + i * 4) * 2);
-            top = max(top, max((x[i].x << 16) & 0x7fff0000u, (x[i].y << 16) & 0x7fff0000u));
-            top = max(top, max(x[i].x & 0x7fff0000u, x[i].y & 0x7fff0000u));
-          }
+        }
+        float back = 1.f;
+        if (!B16) {
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          float f, back;
-          if (CODES == MB_KV_I8) {
+          float f;
+          if (I8) {
             // below 2^-100 the row counts as 0
             const bool some = top >= 0x0d800000u;
             f = some ? 32639.f / __uint_as_float(top) : 0.f;
             back = some ? __uint_as_float(top) / 32639.f : 0.f;
-          } else {
-            const int e = max((int)(top >> 23), 8);
-            f = __uint_as_float((uint32_t)(261 - e) << 23);   // 2^(134 - e)
-            back = __uint_as_float((uint32_t)(e > 8 ? e - 7 : 1) << 23);
+          } else {  // to [1, 2) by a power of two
+            const int e = min(max((int)(top >> 23), 1), 253);
+            f = __uint_as_float((uint32_t)(254 - e) << 23);
+            back = __uint_as_float((uint32_t)e << 23);
           }
           if (top >= 0x7f800000u) f = 0.f, back = __uint_as_float(0x7fc00000u);  // NaN or infinity in the row
-          q_size[r] = back * p.scale_log2;
 #pragma unroll
-          for (int i = 0; i < QW; i++)
-            query_digits<CODES>(x[i], f, digits[r][0][B16 ? 0 : i], digits[r][1][B16 ? 0 : i]);
+          for (int i = 0; i < QW; i++) {
+            if (I8) {
+              uint32_t h, w;
+              query_digits(make_uint2(qa[r][i][0], qa[r][i][1]), f, h, w);
+              qa[r][i][0] = h, qa[r][i][1] = w;
+            } else {
+              qa[r][i][0] = scaled_f16x2(qa[r][i][0], f), qa[r][i][1] = scaled_f16x2(qa[r][i][1], f);
+            }
+          }
         }
+        back *= p.scale_log2;
+        q_size[r][0] = __shfl_sync(0xffffffffu, back, 8 * t), q_size[r][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.f;
+        m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.f;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[d.q_slot]);
-#pragma unroll
-      for (int r = 0; r < RR; r++) {
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.f;
-        m[r] = -INFINITY, l[r] = 0.f;
-      }
       v_ref = v_inv = 0.f;
     }
     const int key0 = warp * 16;
@@ -464,86 +460,79 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
 #pragma unroll
         for (int i = 0; i < D / 32; i++) load_v(i);
       }
-      float sc[2][2 * RR];
+      // scores: sc[r][2 u + e] of key key_of(u, g) and row 8 r + 2t + e
+      const int key_a = S::key_of(0, g), key_b = S::key_of(1, g);
+      float sc[RR][4];
+      int hi[RR][4], lo[RR][4];
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const int key = key0 + S::key_of(u, g);
-        // the lane's bytes of each line: 32 (16 where two rows share a line)
-        constexpr int LB = S::LINEB / 4;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t ch[4] = {0u, 0u, 0u, 0u}, cl[4] = {0u, 0u, 0u, 0u};
+      for (int r = 0; r < RR; r++)
 #pragma unroll
-        for (int pl = 0; pl < S::PLANES; pl++) {
-          uint32_t w[LB / 4];
+        for (int e = 0; e < 4; e++) sc[r][e] = 0.f, hi[r][e] = lo[r][e] = 0;
+      constexpr int LB = S::LINEB / 4;  // a lane's bytes of a row in a line
 #pragma unroll
-          for (int i = 0; i < LB / 16; i++) {
-            const uint4 x = *(const uint4*)(sk + S::at(key, pl * 128 + t * LB + i * 16));
-            w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+      for (int pl = 0; pl < S::PLANES; pl++) {
+        uint32_t wa[LB / 4], wb[LB / 4];
+#pragma unroll
+        for (int i = 0; i < LB / 16; i++) {
+          const uint4 x = *(const uint4*)(sk + S::at(key0 + key_a, pl * 128 + t * LB + i * 16));
+          const uint4 y = *(const uint4*)(sk + S::at(key0 + key_b, pl * 128 + t * LB + i * 16));
+          wa[4 * i] = x.x, wa[4 * i + 1] = x.y, wa[4 * i + 2] = x.z, wa[4 * i + 3] = x.w;
+          wb[4 * i] = y.x, wb[4 * i + 1] = y.y, wb[4 * i + 2] = y.z, wb[4 * i + 3] = y.w;
+        }
+        if (CODES == MB_KV_E4M3) {
+#pragma unroll
+          for (int i = 0; i < LB / 4; i++) {
+            uint32_t a[4];
+            codes_f16<CODES>(wa[i], a[0], a[2]);
+            codes_f16<CODES>(wb[i], a[1], a[3]);
+#pragma unroll
+            for (int r = 0; r < RR; r++) mma16816_f16(sc[r], a[0], a[1], a[2], a[3], qa[r][i][0], qa[r][i][1]);
           }
-          if (B16) {
+        } else {
 #pragma unroll
-            for (int i = 0; i < LB / 8; i++) {
-              const uint32_t* a = qa[B16 ? pl * 4 + i : 0];
-              mma16816(acc, a[0], WIDE ? a[2 * RR - 2] : 0u, a[1], WIDE ? a[2 * RR - 1] : 0u, w[2 * i], w[2 * i + 1]);
-            }
-          } else {
+          for (int i = 0; i < LB / 8; i++)
 #pragma unroll
-            for (int i = 0; i < LB / 8; i++) {
-              const int x = B16 ? 0 : 2 * i, y = B16 ? 0 : 2 * i + 1;
-              if (WIDE) {
-                mma16832<CODES>(ch, digits[0][0][x], digits[RR - 1][0][x], digits[0][0][y], digits[RR - 1][0][y], w[2 * i], w[2 * i + 1]);
-                mma16832<CODES>(cl, digits[0][1][x], digits[RR - 1][1][x], digits[0][1][y], digits[RR - 1][1][y], w[2 * i], w[2 * i + 1]);
-              } else {  // high digits as rows 0-7, low ones as rows 8-15
-                mma16832<CODES>(ch, digits[0][0][x], digits[0][1][x], digits[0][0][y], digits[0][1][y], w[2 * i], w[2 * i + 1]);
+            for (int r = 0; r < RR; r++) {
+              if (B16) {
+                const uint32_t* q = qa[r][B16 ? pl * 4 + i : 0];
+                mma16816(sc[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], q[0], q[1]);
+              } else {
+                const int x = B16 ? 0 : 2 * i, y = B16 ? 0 : 2 * i + 1;
+                mma16832(hi[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], qa[r][x][0], qa[r][y][0]);
+                mma16832(lo[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], qa[r][x][1], qa[r][y][1]);
               }
             }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2 * RR; e++) {
-          if (B16) {
-            sc[u][e] = acc[e];
-          } else {
-            const uint32_t hi = ch[e], lo = WIDE ? cl[e] : ch[e + 2 < 4 ? e + 2 : e];
-            // int8: 256 h + l is below 2^30
-            sc[u][e] = CODES == MB_KV_I8 ? (float)((int)hi * 256 + (int)lo) : __uint_as_float(hi) + __uint_as_float(lo);
-          }
         }
       }
-      float2 vs[2];
-      float mx[RR], ref[RR];
-#pragma unroll
-      for (int r = 0; r < RR; r++) mx[r] = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const int k0 = S::key_of(u, 2 * t);  // and the next one
-        float f0 = 1.f, f1 = 1.f;
-        if (!B16) {
-          const float2 ks = *(const float2*)(sk + 2 * S::KVB + (key0 + k0) * 4);
-          f0 = ks.x, f1 = ks.y;
-          vs[u] = *(const float2*)(sk + 2 * S::KVB + S::SCALEB + (key0 + k0) * 4);
-          if (k0 >= left) vs[u].x = 0.f;  // whatever rows behind the sequence hold
-          if (k0 + 1 >= left) vs[u].y = 0.f;
-        }
-#pragma unroll
-        for (int r = 0; r < RR; r++) {
-          sc[u][2 * r] = k0 < left ? sc[u][2 * r] * (f0 * q_size[r]) : -INFINITY;
-          sc[u][2 * r + 1] = k0 + 1 < left ? sc[u][2 * r + 1] * (f1 * q_size[r]) : -INFINITY;
-          mx[r] = fmaxf(mx[r], fmaxf(sc[u][2 * r], sc[u][2 * r + 1]));
-        }
+      // scales of the two keys; those of rows that do not exist may be anything
+      const bool in_a = key_a < left, in_b = key_b < left;
+      float ks_a = 1.f, ks_b = 1.f, vs_a = 1.f, vs_b = 1.f;
+      if (!B16) {
+        const float* scale = (const float*)(sk + 2 * S::KVB) + key0;
+        ks_a = scale[key_a], ks_b = scale[key_b];
+        vs_a = in_a ? scale[kTileKeys + key_a] : 0.f, vs_b = in_b ? scale[kTileKeys + key_b] : 0.f;
       }
       // The reference points move (and the output with them) only when a score passes its row's by more than 2^kSlack,
       // or a value scale the largest so far.
-      float vm = 0.f;
-      if (!B16) vm = fmaxf(fmaxf(vs[0].x, vs[0].y), fmaxf(vs[1].x, vs[1].y));
-      bool move = vm > v_ref;
+      bool move = !B16 && fmaxf(vs_a, vs_b) > v_ref;
 #pragma unroll
-      for (int r = 0; r < RR; r++) move |= mx[r] > m[r] + kSlack;
+      for (int r = 0; r < RR; r++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          if (I8) {  // below 2^30
+            sc[r][e] = (float)(hi[r][e] * 256 + lo[r][e]);
+            sc[r][2 + e] = (float)(hi[r][2 + e] * 256 + lo[r][2 + e]);
+          }
+          sc[r][e] = in_a ? sc[r][e] * (ks_a * q_size[r][e]) : -INFINITY;
+          sc[r][2 + e] = in_b ? sc[r][2 + e] * (ks_b * q_size[r][e]) : -INFINITY;
+          move |= fmaxf(sc[r][e], sc[r][2 + e]) > m[r][e] + kSlack;
+        }
       if (__any_sync(0xffffffffu, move)) {
         float shrink = 1.f;
         if (!B16) {
-          vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
-          vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
+          float vm = fmaxf(vs_a, vs_b);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, x));
           if (vm > v_ref) {  // the same in all lanes
             shrink = v_ref / vm;
             v_ref = vm;
@@ -552,36 +541,41 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
         }
 #pragma unroll
         for (int r = 0; r < RR; r++) {
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-          const float mn = mx[r] > m[r] + kSlack ? mx[r] : m[r];
-          float alpha = mn == -INFINITY ? 1.f : ex2_approx(m[r] - mn);
-          m[r] = mn;
-          l[r] *= alpha;
-          alpha *= shrink;
-          const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
+          float alpha[2];
 #pragma unroll
-          for (int i = 0; i < D / 16; i++) o[r][i][0] *= a0, o[r][i][1] *= a1, o[r][i][2] *= a0, o[r][i][3] *= a1;
+          for (int e = 0; e < 2; e++) {
+            float mx = fmaxf(sc[r][e], sc[r][2 + e]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float mn = mx > m[r][e] + kSlack ? mx : m[r][e];
+            alpha[e] = mn == -INFINITY ? 1.f : ex2_approx(m[r][e] - mn);
+            m[r][e] = mn;
+            l[r][e] *= alpha[e];
+            alpha[e] *= shrink;
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; i++)
+            o[r][i][0] *= alpha[0], o[r][i][1] *= alpha[1], o[r][i][2] *= alpha[0], o[r][i][3] *= alpha[1];
         }
       }
+      vs_a *= v_inv, vs_b *= v_inv;
+      uint32_t w8[RR][2];  // weights as B operand: keys 8 u + 2t and + 1 of row 8 r + g
 #pragma unroll
-      for (int r = 0; r < RR; r++) ref[r] = m[r] == -INFINITY ? 0.f : m[r];  // nothing but -inf so far: weights 0
-      // The scores' accumulator layout (row g, keys 2t) is that of a B operand with keys as depth: the output is formed
-      // transposed, values as A (16 channels), weights as B (8 rows), and no row of a product is idle.
-      uint32_t w8[RR][2];
+      for (int r = 0; r < RR; r++) {
+        float w[4];
 #pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int r = 0; r < RR; r++) {
-          const float p0 = ex2_approx(sc[u][2 * r] - ref[r]), p1 = ex2_approx(sc[u][2 * r + 1] - ref[r]);
-          l[r] += p0 + p1;
-          if (B16) {
-            w8[r][u] = pack_bf16x2(p0, p1);
-          } else {
-            const __half2 h = __floats2half2_rn(p0 * (vs[u].x * v_inv), p1 * (vs[u].y * v_inv));
-            w8[r][u] = *(const uint32_t*)&h;
-          }
+        for (int e = 0; e < 2; e++) {
+          const float ref = m[r][e] == -INFINITY ? 0.f : m[r][e];  // nothing but -inf so far: weights 0
+          w[e] = ex2_approx(sc[r][e] - ref), w[2 + e] = ex2_approx(sc[r][2 + e] - ref);
+          l[r][e] += w[e] + w[2 + e];
         }
+        if (B16) {
+          w8[r][0] = movmatrix(pack_bf16x2(w[0], w[1])), w8[r][1] = movmatrix(pack_bf16x2(w[2], w[3]));
+        } else {
+          const __half2 a = __floats2half2_rn(w[0] * vs_a, w[1] * vs_a), b = __floats2half2_rn(w[2] * vs_b, w[3] * vs_b);
+          w8[r][0] = movmatrix(*(const uint32_t*)&a), w8[r][1] = movmatrix(*(const uint32_t*)&b);
+        }
+      }
       if (B16) {
         // values that do not exist may be NaN: zero their rows first (a tile's partial last group only)
         if (left < 16) {
@@ -630,11 +624,13 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     const int hk = d.unit / p.q_tiles, qt = d.unit - hk * p.q_tiles;
     const int rows = min(kRows, p.G - qt * kRows), head0 = hk * p.G + qt * kRows;
 #pragma unroll
-    for (int r = 0; r < RR; r++) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t == 0) s_m[warp * kRows + g + 8 * r] = m[r], s_l[warp * kRows + g + 8 * r] = l[r];
-    }
+    for (int r = 0; r < RR; r++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], x);
+        if (g == 0) s_m[warp * kRows + 8 * r + 2 * t + e] = m[r][e], s_l[warp * kRows + 8 * r + 2 * t + e] = l[r][e];
+      }
     if (lane == 0) s_v[warp] = B16 ? 1.f : v_ref / kWeightOne;
     bool ok = true;
     auto meet = [&] {  // of the four warps
