@@ -680,27 +680,60 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
   }
 }
 
-// Adds up the parts of each unit that several blocks hold. One block a unit and row.
+// Adds up the parts of each unit that several blocks hold, in the blocks' order; one block for each unit and query row.
+// Launched while k_attention_paged still runs (programmatic launch): it waits for that grid before it reads anything.
+constexpr int kJoinWarps = 4;
 template <int D>
-__global__ void __launch_bounds__(D) k_join(const Params p) {
-  const int u = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
+__global__ void __launch_bounds__(32 * kJoinWarps) k_join(const Params p) {
+  __shared__ float4 s_acc[kJoinWarps][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int u = blockIdx.x, r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = u / p.units_per_seq, unit = u - b * p.units_per_seq;
   const int hk = unit / p.q_tiles, qt = unit - hk * p.q_tiles;
-  if (r >= p.G - qt * kRows || __ldg(p.lens + b) <= 0 || p.table_width == 0) return;
+  if (r >= p.G - qt * kRows || p.table_width == 0) return;
+  const int len = __ldg(p.lens + b);
   const Part part = p.parts[u];
-  if (part.pieces <= 1) return;
+  if (len <= 0 || part.pieces <= 1) return;
   auto slot = [&](int i) { return (int64_t)2 * (part.first + i) + (i == 0 ? 1 : 0); };
+  // every warp the statistics of all parts, 32 at a time
   float top = -INFINITY;
-  for (int i = 0; i < part.pieces; i++) top = fmaxf(top, p.part_ml[slot(i) * 2 * kRows + r]);
+  for (int i = lane; i < part.pieces; i += 32) top = fmaxf(top, p.part_ml[slot(i) * 2 * kRows + r]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float ref = top == -INFINITY ? 0.f : top;
-  float acc = 0.f, sum = 0.f;
-  for (int i = 0; i < part.pieces; i++) {
-    const int64_t s = slot(i);
-    const float f = ex2_approx(p.part_ml[s * 2 * kRows + r] - ref);
-    acc += f * p.part_o[(s * kRows + r) * D + d];
-    sum += f * p.part_ml[s * 2 * kRows + kRows + r];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int i0 = 0; i0 < part.pieces; i0 += 32) {
+    const int n = min(32, part.pieces - i0);
+    float f = 0.f;
+    if (lane < n) {
+      f = ex2_approx(p.part_ml[slot(i0 + lane) * 2 * kRows + r] - ref);
+      sum += f * p.part_ml[slot(i0 + lane) * 2 * kRows + kRows + r];
+    }
+#pragma unroll 8
+    for (int i = warp; i < n; i += kJoinWarps) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      if (lane < D / 4) {
+        const float4 x = *((const float4*)(p.part_o + (slot(i0 + i) * kRows + r) * D) + lane);
+        acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w;
+      }
+    }
   }
-  p.out[(int64_t)b * p.ldo + (int64_t)(hk * p.G + qt * kRows + r) * D + d] = __float2bfloat16_rn(acc / sum);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  s_acc[warp][lane] = acc;
+  __syncthreads();
+  if (warp == 0 && lane < D / 4) {
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; w++) {
+      const float4 x = s_acc[w][lane];
+      acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    }
+    uint2 y;
+    y.x = pack_bf16x2(acc.x / sum, acc.y / sum);
+    y.y = pack_bf16x2(acc.z / sum, acc.w / sum);
+    *((uint2*)(p.out + (int64_t)b * p.ldo + (int64_t)(hk * p.G + qt * kRows + r) * D) + lane) = y;
+  }
 }
 
 struct Layout {
@@ -745,8 +778,18 @@ template <int CODES, int D>
 cudaError_t launch(const Params& p, int64_t units, cudaStream_t st) {
   cudaError_t e = p.G > 8 ? launch_attention<CODES, D, true>(p, st) : launch_attention<CODES, D, false>(p, st);
   if (e != cudaSuccess) return e;
-  k_join<D><<<dim3((unsigned)units, (unsigned)(p.G < kRows ? p.G : kRows)), D, 0, st>>>(p);
-  return cudaGetLastError();
+  // a unit that fits a tile is never split
+  if (((int64_t)p.table_width << p.c.page_log2) <= kTileKeys) return cudaSuccess;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)units, (unsigned)(p.G < kRows ? p.G : kRows));
+  cfg.blockDim = dim3(32 * kJoinWarps);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_join<D>, p);
 }
 
 }  // namespace paged
