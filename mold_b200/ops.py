@@ -281,21 +281,17 @@ def gguf_inspect(path):
 
 
 # ---------------------------------------------------------------- text transformers
+# A generation step makes hundreds of these calls, so the checks are kept to a few attribute reads each.
 
-def _ready(*tensors):
+def _ready(first, *others):
     """The one device of the tensors (None ones aside), initialised, as an index."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("tensors must be CUDA tensors")
-        d = t.device.index
-        if dev is None:
-            dev = d
-        elif dev != d:
-            raise ValueError(f"tensors on devices {dev} and {d}")
+    dev = first.get_device()  # -1 on the CPU
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on different devices ({first.device} and {t.device})")
     if dev not in _inited:
+        if dev < 0:
+            raise ValueError("tensors must be CUDA tensors")
         with torch.cuda.device(dev):
             check(lib().mb_init(dev))
         _inited.add(dev)
@@ -304,43 +300,58 @@ def _ready(*tensors):
 
 def _launch(dev, fn, *args):
     """fn(*args, stream) on device `dev` and its current stream, whichever device is current."""
-    st = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    if dev == torch.cuda.current_device():
-        return check(fn(*args, st))
-    with torch.cuda.device(dev):
-        return check(fn(*args, st))
+    st = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        status = fn(*args, st)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, st)
+    if status:
+        check(status)
 
 
 def _heads(x, name, copy=True):
-    """(x, row stride) of a bf16 [rows, heads, D] tensor whose rows are whole and 16-byte aligned; a tensor laid out
-    otherwise is copied, or with copy=False refused."""
-    if x.dim() != 3 or x.dtype != torch.bfloat16:
+    """(x, address, row stride, rows, heads, head size) of a bf16 [rows, heads, D] tensor whose rows are whole and
+    16-byte aligned; a tensor laid out otherwise is copied, or with copy=False refused."""
+    if x.dtype is not torch.bfloat16 or x.dim() != 3:
         raise ValueError(f"{name} must be bf16 [rows, heads, head_dim], got {x.dtype} {tuple(x.shape)}")
     rows, h, d = x.shape
-    s0, s1, s2 = x.stride()
-    if not (s2 == 1 and (h == 1 or s1 == d) and (rows <= 1 or (s0 >= h * d and s0 % 8 == 0))
-            and x.data_ptr() % 16 == 0):
-        if not copy:
-            raise ValueError(f"{name} must have whole rows, 16-byte aligned (strides {x.stride()})")
-        x = x.clone(memory_format=torch.contiguous_format)
-        s0 = h * d
-    return x, (s0 if rows > 1 else h * d)
+    ptr = x.data_ptr()
+    if ptr & 15 == 0:
+        if x.is_contiguous():
+            return x, ptr, h * d, rows, h, d
+        s0, s1, s2 = x.stride()
+        if s2 == 1 and (h == 1 or s1 == d) and (rows <= 1 or (s0 >= h * d and s0 & 7 == 0)):
+            return x, ptr, (s0 if rows > 1 else h * d), rows, h, d
+    if not copy:
+        raise ValueError(f"{name} must have whole rows, 16-byte aligned (strides {x.stride()})")
+    x = x.clone(memory_format=torch.contiguous_format)
+    return x, x.data_ptr(), h * d, rows, h, d
 
 
-def _ints(x, name, dim=1):
-    if x.dtype != torch.int32 or x.dim() != dim or (x.numel() and x.stride(-1) != 1 and x.shape[-1] > 1):
-        raise ValueError(f"{name} must be int32 with {dim} dimension(s) and contiguous rows, got {x.dtype} "
-                         f"{tuple(x.shape)}")
-    return x
+def _ints(x, name, n=None):
+    """(x's address, entries) of an int32 vector, of n entries where n is given."""
+    if x.dtype is not torch.int32 or x.dim() != 1 or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector, got {x.dtype} {tuple(x.shape)}")
+    m = x.shape[0]
+    if n is not None and m != n:
+        raise ValueError(f"{name} has {m} entries, expected {n}")
+    return x.data_ptr(), m
 
 
 def _table(table, n_seqs):
-    _ints(table, "table", 2)
-    if table.shape[0] != n_seqs:
-        raise ValueError(f"table has {table.shape[0]} rows for {n_seqs} sequences")
-    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
-        table = table.contiguous()
-    return table, (table.stride(0) if table.shape[0] > 1 else table.shape[1])
+    """(table, address, row stride, pages a row) of an int32 page table of n_seqs rows."""
+    if table.dtype is not torch.int32 or table.dim() != 2:
+        raise ValueError(f"table must be int32 [sequences, pages], got {table.dtype} {tuple(table.shape)}")
+    n, width = table.shape
+    if n != n_seqs:
+        raise ValueError(f"table has {n} rows for {n_seqs} sequences")
+    ld = width
+    if not table.is_contiguous():
+        ld, s1 = table.stride()
+        if n <= 1 or (width > 1 and s1 != 1) or ld < width:
+            table, ld = table.contiguous(), width
+    return table, table.data_ptr(), ld, width
 
 
 def _scale(scale):
@@ -358,22 +369,29 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
     the last sequence are not written."""
     cu_k = cu_q if cu_k is None else cu_k
     dev = _ready(q, k, v, cu_q, cu_k, out)
-    (q, ldq), (k, ldk), (v, ldv) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
-    tq, h, d = q.shape
-    if k.shape != v.shape or k.shape[2] != d:
+    q, q_ptr, ldq, tq, h, d = _heads(q, "q")
+    k, k_ptr, ldk, tk, hk, dk = _heads(k, "k")
+    v, v_ptr, ldv, tv, hv, dv = _heads(v, "v")
+    if tk != tv or hk != hv or dk != d or dv != d:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
-    _ints(cu_q, "cu_q"), _ints(cu_k, "cu_k")
-    if cu_q.numel() < 1 or cu_k.numel() != cu_q.numel():
-        raise ValueError("cu_q and cu_k must both have one entry more than there are sequences")
-    if out is None:
-        out = torch.empty((tq, h, d), dtype=torch.bfloat16, device=q.device)
-    elif out.shape != q.shape:
-        raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
-    out, ldo = _heads(out, "out", copy=False)
-    _launch(dev, lib().mb_attention_varlen, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, tq, k.shape[0], h,
-            k.shape[1], d, cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, int(bool(causal)), _scale(scale),
-            out.data_ptr(), ldo)
+    cq_ptr, n = _ints(cu_q, "cu_q")
+    ck_ptr, _ = _ints(cu_k, "cu_k", n)
+    if n < 1:
+        raise ValueError("cu_q must have one entry more than there are sequences")
+    out, o_ptr, ldo = _out(out, q)
+    _launch(dev, lib().mb_attention_varlen, q_ptr, ldq, k_ptr, ldk, v_ptr, ldv, tq, tk, h, hk, d, cq_ptr, ck_ptr, n - 1,
+            1 if causal else 0, _scale(scale), o_ptr, ldo)
     return out
+
+
+def _out(out, q):
+    """(out, address, row stride): the caller's tensor, or a new one, shaped like q."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        return out, out.data_ptr(), q.shape[1] * q.shape[2]
+    if out.shape != q.shape:
+        raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
+    return _heads(out, "out", copy=False)[:3]
 
 
 _KV_TYPES = {torch.bfloat16: KV_BF16, torch.int8: KV_I8, torch.float8_e4m3fn: KV_E4M3}
@@ -419,34 +437,46 @@ class KVCache:
         self._c = KVCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
                            v_scale.data_ptr() if v_scale is not None else None, self.n_pages, self.page_size,
                            self.n_kv_heads, self.head_dim, _KV_TYPES[k.dtype])
+        self._ref = ctypes.byref(self._c)
+        self._workspaces = {}
+
+    def _workspace_bytes(self, n_seqs, heads):
+        """mb_attention_paged_workspace for n_seqs sequences of `heads` query heads (a function of these sizes)."""
+        got = self._workspaces.get((n_seqs, heads))
+        if got is None:
+            nbytes = ctypes.c_size_t(0)
+            check(lib().mb_attention_paged_workspace(n_seqs, heads, self.n_kv_heads, self.head_dim,
+                                                     ctypes.byref(nbytes)))
+            got = self._workspaces[n_seqs, heads] = nbytes.value
+        return got
 
     def _rows(self, x, name, copy=True):
-        x, ld = _heads(x, name, copy)
-        if x.shape[1:] != (self.n_kv_heads, self.head_dim):
+        x, ptr, ld, rows, h, d = _heads(x, name, copy)
+        if h != self.n_kv_heads or d != self.head_dim:
             raise ValueError(f"{name} is {tuple(x.shape)}, the cache has {self.n_kv_heads} heads of {self.head_dim}")
-        return x, ld
+        return x, ptr, ld, rows
 
     def write(self, k, v, table, kv_lens, cu=None):
         """Append rows k, v (bf16 [T, n_kv_heads, head_dim]): sequence b's rows [cu[b], cu[b+1]) become its last
         positions, kv_lens[b] (int32, the length after the call) at their end. Without cu, row b is sequence b's one
         new position, and a sequence with kv_lens[b] <= 0 gets none."""
         dev = _ready(self.k, k, v, table, kv_lens, cu)
-        (k, ldk), (v, ldv) = self._rows(k, "k"), self._rows(v, "v")
-        if k.shape != v.shape:
+        k, k_ptr, ldk, rows = self._rows(k, "k")
+        v, v_ptr, ldv, v_rows = self._rows(v, "v")
+        if rows != v_rows:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-        n = _ints(kv_lens, "kv_lens").numel()
-        if cu is not None and _ints(cu, "cu").numel() != n + 1:
-            raise ValueError(f"cu has {cu.numel()} entries for {n} sequences")
-        table, ldt = _table(table, n)
-        _launch(dev, lib().mb_kv_write, ctypes.byref(self._c), k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[0],
-                None if cu is None else cu.data_ptr(), kv_lens.data_ptr(), table.data_ptr(), ldt, table.shape[1], n)
+        lens_ptr, n = _ints(kv_lens, "kv_lens")
+        cu_ptr = None if cu is None else _ints(cu, "cu", n + 1)[0]
+        table, t_ptr, ldt, width = _table(table, n)
+        _launch(dev, lib().mb_kv_write, self._ref, k_ptr, ldk, v_ptr, ldv, rows, cu_ptr, lens_ptr, t_ptr, ldt, width, n)
 
     def read(self, table, cu, n_tokens=None, k=None, v=None):
         """The first cu[b+1] - cu[b] positions of each sequence, packed: k, v bf16 [n_tokens, n_kv_heads, head_dim].
         n_tokens (default: cu's last entry, which waits for the device) or k and v give the size; rows behind the last
         sequence are not written."""
         dev = _ready(self.k, table, cu, k, v)
-        n = _ints(cu, "cu").numel() - 1
+        cu_ptr, n = _ints(cu, "cu")
+        n -= 1
         if n < 0:
             raise ValueError("cu must have one entry more than there are sequences")
         if (k is None) != (v is None):
@@ -454,13 +484,14 @@ class KVCache:
         if k is None:
             n_tokens = int(cu[-1]) if n_tokens is None else int(n_tokens)
             shape = (n_tokens, self.n_kv_heads, self.head_dim)
-            k, v = (torch.empty(shape, dtype=torch.bfloat16, device=self.k.device) for _ in range(2))
-        (k, ldk), (v, ldv) = self._rows(k, "k", copy=False), self._rows(v, "v", copy=False)
-        if k.shape != v.shape or (n_tokens is not None and n_tokens != k.shape[0]):
+            k = torch.empty(shape, dtype=torch.bfloat16, device=self.k.device)
+            v = torch.empty(shape, dtype=torch.bfloat16, device=self.k.device)
+        k, k_ptr, ldk, rows = self._rows(k, "k", copy=False)
+        v, v_ptr, ldv, v_rows = self._rows(v, "v", copy=False)
+        if rows != v_rows or (n_tokens is not None and n_tokens != rows):
             raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} and n_tokens {n_tokens} do not fit")
-        table, ldt = _table(table, n)
-        _launch(dev, lib().mb_kv_read, ctypes.byref(self._c), cu.data_ptr(), table.data_ptr(), ldt, table.shape[1], n,
-                k.shape[0], k.data_ptr(), ldk, v.data_ptr(), ldv)
+        table, t_ptr, ldt, width = _table(table, n)
+        _launch(dev, lib().mb_kv_read, self._ref, cu_ptr, t_ptr, ldt, width, n, rows, k_ptr, ldk, v_ptr, ldv)
         return k, v
 
 
@@ -468,23 +499,16 @@ def attention_paged(q, cache: KVCache, table, kv_lens, scale=None, out=None):
     """Attention of one new token of each sequence over its cached positions 0 .. kv_lens[b] - 1: q [B, H, D] bf16 ->
     out [B, H, D]; a sequence without positions gives 0. Equal calls give equal bits."""
     dev = _ready(cache.k, q, table, kv_lens, out)
-    q, ldq = _heads(q, "q")
-    n, h, d = q.shape
+    q, q_ptr, ldq, n, h, d = _heads(q, "q")
     if d != cache.head_dim:
         raise ValueError(f"q has head_dim {d}, the cache {cache.head_dim}")
-    if _ints(kv_lens, "kv_lens").numel() != n:
-        raise ValueError(f"kv_lens has {kv_lens.numel()} entries for {n} sequences")
-    table, ldt = _table(table, n)
-    if out is None:
-        out = torch.empty((n, h, d), dtype=torch.bfloat16, device=q.device)
-    elif out.shape != q.shape:
-        raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
-    out, ldo = _heads(out, "out", copy=False)
-    nbytes = ctypes.c_size_t(0)
-    check(lib().mb_attention_paged_workspace(n, h, cache.n_kv_heads, d, ctypes.byref(nbytes)))
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
-    _launch(dev, lib().mb_attention_paged, q.data_ptr(), ldq, ctypes.byref(cache._c), kv_lens.data_ptr(),
-            table.data_ptr(), ldt, table.shape[1], n, h, _scale(scale), out.data_ptr(), ldo, ws.data_ptr(), nbytes.value)
+    lens_ptr, _ = _ints(kv_lens, "kv_lens", n)
+    table, t_ptr, ldt, width = _table(table, n)
+    out, o_ptr, ldo = _out(out, q)
+    nbytes = cache._workspace_bytes(n, h)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)  # of this call alone: the stream's, or the graph's
+    _launch(dev, lib().mb_attention_paged, q_ptr, ldq, cache._ref, lens_ptr, t_ptr, ldt, width, n, h, _scale(scale),
+            o_ptr, ldo, ws.data_ptr(), nbytes)
     return out
 
 
