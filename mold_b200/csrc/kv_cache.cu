@@ -1,9 +1,10 @@
 // K12 / K13: the paged key-value cache of a text transformer, written (bf16, or 8-bit codes with
 // one f32 scale for each row of head_dim values) and read back.
 //
-// Both move each row once: a group of head_dim / 8 threads owns a (token, head) row of k and the
-// same row of v, 16 bytes of bf16 a thread. Bound by HBM.
-#include <mutex>
+// A group of head_dim / 16 threads owns a (token, head) row of k and the same row of v, two times 16 bytes
+// of bf16 a thread; a warp walks kRows rows of each group, so that the search for the sequence is made once
+// and every load of the warp is in flight before the first is used. Bound by HBM, with little to spare for
+// instructions: hence packed f32 arithmetic and no integer conversions or divisions.
 #include <string>
 
 #include "common.cuh"
@@ -13,15 +14,61 @@
 namespace mb {
 namespace kv {
 
-// The sequence whose rows hold t: the last b with cu[b] <= t. Whatever cu holds, b is in [0, n).
+constexpr int kRows = 2;   // rows a group handles
+constexpr int kHalves = 2;  // 16-byte pieces of a bf16 row that a thread holds, half a row apart
+
+// The sequence whose rows hold t: the last b with cu[b] <= t. All lanes of the warp with the same t; 32 entries a step.
+// Whatever cu holds, b is in [0, n).
 MB_DEV int seq_of(const int32_t* cu, int n, int64_t t) {
-  int lo = 0, hi = n;  // cu[lo] <= t < cu[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) >> 5, at = lane * step;
+    const unsigned le = __ballot_sync(0xffffffffu, at < n && __ldg(cu + lo + (at < n ? at : 0)) <= t);
+    const int k = max(__popc(le), 1) - 1;  // le is a run of ones from bit 0
+    lo += k * step;
+    n = min(step, n - k * step);
   }
   return lo;
 }
+
+MB_DEV uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1,%2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+MB_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MB_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+MB_DEV void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0,%1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+MB_DEV uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// The row of a warp's first group, and a step from it to the next of a group's rows.
+struct Walk {
+  int64_t t;
+  int h, heads;
+  MB_DEV Walk(int64_t row, int heads_) : heads(heads_) {
+    t = row < (1LL << 32) ? (int64_t)((uint32_t)row / (uint32_t)heads_) : row / heads_;
+    h = (int)(row - t * heads_);
+  }
+  MB_DEV bool next(int by) {  // whether the token changed
+    h += by;
+    if (h < heads) return false;
+    while (h >= heads) h -= heads, t++;
+    return true;
+  }
+};
 
 struct WriteParams {
   Cache c;
@@ -33,90 +80,142 @@ struct WriteParams {
   int* status;
 };
 
-// A row's eight values of this thread as codes; scale: what the row's codes stand for times.
+// fl(T / m) and fl(m / T) for a positive bf16 number m (bits `top` of the f32) from 2^-100 on. Both are scaled by powers
+// of two from m in [1, 2), where one correction by the remainder (Markstein's) rounds the quotient correctly; the tests
+// compare all 128 fractions with division.
+template <int CODES>
+MB_DEV void scales_of(uint32_t top, float& s, float& r) {
+  constexpr float T = CODES == MB_KV_I8 ? 127.f : 448.f, IT = 1.f / T;
+  const uint32_t e = (top & 0x7f800000u) - 0x3f800000u;  // exponent, to be added to an f32's bits
+  const float f = __uint_as_float(top - e);
+  float q = f * IT;
+  q = fmaf(fmaf(-q, T, f), IT, q);
+  s = __uint_as_float(__float_as_uint(q) + e);
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(f));
+  float z = T * y;
+  z = fmaf(fmaf(-z, f, T), y, z);
+  r = __uint_as_float(__float_as_uint(z) - e);
+}
+
+// A row's values of this thread as codes, and the row's scale.
 template <int CODES, int GROUP>
-MB_DEV uint2 encode_row(const uint4& x, float& scale) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  // largest magnitude: the bit patterns of non-negative floats order like the floats, NaN last
+MB_DEV void encode_row(const uint4 (&x)[kHalves], uint2 (&out)[kHalves], float& scale) {
+  // largest magnitude: the bit patterns of non-negative bf16 numbers order like the numbers, NaN last
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) top = max(top, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+  for (int i = 0; i < kHalves; i++) {
+    top = max_u16x2(top, max_u16x2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu));
+    top = max_u16x2(top, max_u16x2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+  }
 #pragma unroll
-  for (int o = GROUP / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr float T = CODES == MB_KV_I8 ? 127.f : 448.f;
-  const bool finite = top < 0x7f800000u;
-  const bool some = finite && top >= 0x0d800000u;  // 2^-100: below it the inverse would overflow
-  const float m = __uint_as_float(top);
-  scale = some ? __fdiv_rn(m, T) : finite ? 0.f : __uint_as_float(0x7fc00000u);
-  const float r = some ? __fdiv_rn(T, m) : 0.f;
-  uint32_t out[2];
+  for (int o = GROUP / 2; o; o >>= 1) top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
+  top = max(top << 16, top & 0xffff0000u);
+  float r;
+  scales_of<CODES>(top, scale, r);
+  if (top - 0x0d800000u >= 0x7f800000u - 0x0d800000u) {  // below 2^-100, or not finite: then any code reads back as NaN
+    r = 0.f;
+    scale = top < 0x0d800000u ? 0.f : __uint_as_float(0x7fc00000u);
+  }
+  const uint64_t r2 = pack2(r, r);
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    float y[4];
+  for (int i = 0; i < kHalves; i++) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    uint32_t o[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      y[2 * j] = __fmul_rn(bf16_lo(w[2 * i + j]), r);
-      y[2 * j + 1] = __fmul_rn(bf16_hi(w[2 * i + j]), r);
+      uint64_t a = mul2(pack2(bf16_lo(w[2 * j]), bf16_hi(w[2 * j])), r2);
+      uint64_t b = mul2(pack2(bf16_lo(w[2 * j + 1]), bf16_hi(w[2 * j + 1])), r2);
+      float y0, y1, y2, y3;
+      if (CODES == MB_KV_I8) {
+        // |y| <= 127 (1 + 2^-23); adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the
+        // low byte (the conversion instruction runs at a quarter of the rate). Scalar additions: a packed one after the
+        // packed product came out as one fused operation, without the product's rounding, and took ties the wrong way.
+        unpack2(a, y0, y1), unpack2(b, y2, y3);
+        const uint32_t v0 = __float_as_uint(__fadd_rn(y0, 12582912.f)), v1 = __float_as_uint(__fadd_rn(y1, 12582912.f));
+        const uint32_t v2 = __float_as_uint(__fadd_rn(y2, 12582912.f)), v3 = __float_as_uint(__fadd_rn(y3, 12582912.f));
+        o[j] = __byte_perm(__byte_perm(v0, v1, 0x0040), __byte_perm(v2, v3, 0x0040), 0x5410);
+      } else {
+        uint16_t lo, hi;
+        unpack2(a, y0, y1), unpack2(b, y2, y3);
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y1), "f"(y0));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y3), "f"(y2));
+        o[j] = (uint32_t)lo | ((uint32_t)hi << 16);
+      }
     }
-    if (!finite) y[0] = y[1] = y[2] = y[3] = 0.f;  // NaN and infinity times 0
-    if (CODES == MB_KV_I8) {
-      // |y| <= 127 (1 + 2^-23) rounds to at most 127
-      uint32_t b = 0;
-#pragma unroll
-      for (int j = 0; j < 4; j++) b |= ((uint32_t)__float2int_rn(y[j]) & 255u) << (8 * j);
-      out[i] = b;
-    } else {
-      uint16_t lo, hi;
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
-      out[i] = (uint32_t)lo | ((uint32_t)hi << 16);
-    }
+    out[i] = make_uint2(o[0], o[1]);
   }
-  return make_uint2(out[0], out[1]);
 }
 
 template <int CODES, int D>
 __global__ void __launch_bounds__(256) k_kv_write(const WriteParams p) {
-  constexpr int GROUP = D / 8;
-  const int lane = threadIdx.x % GROUP;
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / GROUP;
-  const int heads = p.c.heads;
-  const int64_t t = row / heads;
-  const int h = (int)(row - t * heads);
-  int64_t dst = -1;
-  if (t < p.n_tokens) {
-    int b = (int)t;
-    int64_t pos = 0, first = 0;
-    if (p.cu) {
-      b = seq_of(p.cu, p.n_seqs, t);
-      const int64_t c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
-      first = (t >= c0 && t < c1) ? t - c1 : INT64_MIN / 2;
-    } else {
-      first = -1;
+  constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
+  const int lane = threadIdx.x % GROUP, side = (threadIdx.x & 31) / GROUP;
+  const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (SIDE * kRows);  // the warp's
+  if (row0 >= p.n_tokens * p.c.heads) return;
+  const Walk first(row0, p.c.heads);
+  Walk w = first;
+  w.next(side);
+  const Walk own = w;
+  uint4 kx[kRows][kHalves], vx[kRows][kHalves];
+#pragma unroll
+  for (int i = 0; i < kRows; i++) {
+    const uint4* ks = (const uint4*)(p.k + w.t * p.ldk + w.h * D) + lane;
+    const uint4* vs = (const uint4*)(p.v + w.t * p.ldv + w.h * D) + lane;
+#pragma unroll
+    for (int j = 0; j < kHalves; j++) {
+      kx[i][j] = vx[i][j] = make_uint4(0, 0, 0, 0);
+      if (w.t < p.n_tokens) kx[i][j] = ld_stream(ks + j * GROUP), vx[i][j] = ld_stream(vs + j * GROUP);
     }
-    pos = (int64_t)__ldg(p.lens + b) + first;
-    if (pos >= 0) dst = row_of(p.c, p.table + (int64_t)b * p.ld_table, p.table_width, pos, h, p.status);
+    w.next(SIDE);
   }
-  // whole groups agree on dst; the shuffles below need every lane of the warp
-  uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  if (dst >= 0) {
-    kx = ld_stream((const uint4*)(p.k + t * p.ldk + (int64_t)h * D) + lane);
-    vx = ld_stream((const uint4*)(p.v + t * p.ldv + (int64_t)h * D) + lane);
-  }
-  if (CODES == MB_KV_BF16) {
-    if (dst >= 0) {
-      ((uint4*)p.c.k)[dst * GROUP + lane] = kx;
-      ((uint4*)p.c.v)[dst * GROUP + lane] = vx;
+  // places in the cache, while the rows are on their way
+  int64_t dst[kRows], base = -1;
+  int b = p.cu ? seq_of(p.cu, p.n_seqs, first.t) : 0;
+  int64_t c1 = p.cu ? (int64_t)__ldg(p.cu + b + 1) : 0;
+  w = own;
+  bool moved = true;
+#pragma unroll
+  for (int i = 0; i < kRows; i++) {
+    if (moved) {
+      base = -1;
+      if (w.t < p.n_tokens) {
+        int64_t pos;
+        if (p.cu) {
+          while (w.t >= c1 && b + 1 < p.n_seqs) c1 = __ldg(p.cu + ++b + 1);
+          pos = w.t < c1 && w.t >= __ldg(p.cu + b) ? (int64_t)__ldg(p.lens + b) - (c1 - w.t) : -1;
+        } else {
+          b = (int)w.t;
+          pos = (int64_t)__ldg(p.lens + b) - 1;
+        }
+        if (pos >= 0) base = row_of(p.c, p.table + (int64_t)b * p.ld_table, p.table_width, pos, 0, p.status);
+      }
     }
-  } else {
-    float ks, vs;
-    const uint2 kc = encode_row<CODES, GROUP>(kx, ks), vc = encode_row<CODES, GROUP>(vx, vs);
-    if (dst >= 0) {
-      ((uint2*)p.c.k)[dst * GROUP + lane] = kc;
-      ((uint2*)p.c.v)[dst * GROUP + lane] = vc;
-      if (lane == 0) {
-        p.c.k_scale[dst] = ks;
-        p.c.v_scale[dst] = vs;
+    dst[i] = base < 0 ? -1 : base + ((int64_t)w.h << p.c.page_log2);
+    moved = w.next(SIDE);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; i++) {
+    if (CODES == MB_KV_BF16) {
+      if (dst[i] >= 0)
+#pragma unroll
+        for (int j = 0; j < kHalves; j++) {
+          ((uint4*)p.c.k)[dst[i] * (D / 8) + j * GROUP + lane] = kx[i][j];
+          ((uint4*)p.c.v)[dst[i] * (D / 8) + j * GROUP + lane] = vx[i][j];
+        }
+    } else {  // shuffles inside: every lane
+      float ks, vs;
+      uint2 kc[kHalves], vc[kHalves];
+      encode_row<CODES, GROUP>(kx[i], kc, ks);
+      encode_row<CODES, GROUP>(vx[i], vc, vs);
+      if (dst[i] >= 0) {
+#pragma unroll
+        for (int j = 0; j < kHalves; j++) {
+          ((uint2*)p.c.k)[dst[i] * (D / 8) + j * GROUP + lane] = kc[j];
+          ((uint2*)p.c.v)[dst[i] * (D / 8) + j * GROUP + lane] = vc[j];
+        }
+        if (lane == 0) p.c.k_scale[dst[i]] = ks;
+        if (lane == 1) p.c.v_scale[dst[i]] = vs;
       }
     }
   }
@@ -133,45 +232,110 @@ struct ReadParams {
   int* status;
 };
 
+// Two numbers that codes 2 i and 2 i + 1 of a word stand for (before the scale), exactly.
+template <int CODES>
+MB_DEV uint64_t decode2(uint32_t w, int i) {
+  if (CODES == MB_KV_I8) {
+    // byte c + 128 in the last place of 2^23
+    const uint32_t u = w ^ 0x80808080u;
+    return add2(pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + 2 * i)),
+                      __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7651 + 2 * i))),
+                pack2(-8388736.f, -8388736.f));
+  }
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (16 * i))));
+  const float2 f = __half22float2(*(const __half2*)&h);
+  return pack2(f.x, f.y);
+}
+
+template <int CODES>
+struct Held {  // a thread's values of a row as the cache holds them
+  uint4 x[kHalves];
+  float s;
+};
 template <int CODES, int D>
-MB_DEV uint4 decode_row(const void* base, const float* scales, int64_t src, int lane) {
-  constexpr int GROUP = D / 8;
-  if (CODES == MB_KV_BF16) return ld_stream((const uint4*)base + src * GROUP + lane);
-  const uint2 c = ld_stream((const uint2*)base + src * GROUP + lane);
-  const float s = __ldg(scales + src);
-  const uint32_t w[2] = {c.x, c.y};
+MB_DEV void load_row(Held<CODES>& r, const void* base, const float* scales, int64_t src, int lane) {
+  constexpr int GROUP = D / 16;
+  r.s = 0.f;
+#pragma unroll
+  for (int j = 0; j < kHalves; j++) {
+    r.x[j] = make_uint4(0, 0, 0, 0);
+    if (src < 0) continue;
+    if (CODES == MB_KV_BF16) {
+      r.x[j] = ld_stream((const uint4*)base + src * (D / 8) + j * GROUP + lane);
+    } else {
+      const uint2 c = ld_stream((const uint2*)base + src * (D / 8) + j * GROUP + lane);
+      r.x[j].x = c.x, r.x[j].y = c.y;
+    }
+  }
+  if (CODES != MB_KV_BF16 && src >= 0) r.s = __ldg(scales + src);
+}
+template <int CODES>
+MB_DEV uint4 decode_row(const Held<CODES>& r, int j) {
+  if (CODES == MB_KV_BF16) return r.x[j];
+  const uint64_t s2 = pack2(r.s, r.s);
   uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    float y[4];
-    decode4<CODES>(w[i], y);
+  for (int i = 0; i < 4; i++) {
     // f32 product, then one rounding to bf16
-    o[2 * i] = pack_bf16x2(__fmul_rn(y[0], s), __fmul_rn(y[1], s));
-    o[2 * i + 1] = pack_bf16x2(__fmul_rn(y[2], s), __fmul_rn(y[3], s));
+    float a, b;
+    unpack2(mul2(decode2<CODES>(i < 2 ? r.x[j].x : r.x[j].y, i & 1), s2), a, b);
+    o[i] = pack_bf16x2(a, b);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 template <int CODES, int D>
 __global__ void __launch_bounds__(256) k_kv_read(const ReadParams p) {
-  constexpr int GROUP = D / 8;
-  const int lane = threadIdx.x % GROUP;
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / GROUP;
-  const int heads = p.c.heads;
-  const int64_t t = row / heads;
-  const int h = (int)(row - t * heads);
-  if (t >= p.n_tokens) return;
-  const int b = seq_of(p.cu, p.n_seqs, t);
-  const int64_t c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
-  if (t < c0 || t >= c1) return;
-  const int64_t src = row_of(p.c, p.table + (int64_t)b * p.ld_table, p.table_width, t - c0, h, p.status);
-  uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-  if (src >= 0) {
-    kx = decode_row<CODES, D>(p.c.k, p.c.k_scale, src, lane);
-    vx = decode_row<CODES, D>(p.c.v, p.c.v_scale, src, lane);
+  constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
+  const int lane = threadIdx.x % GROUP, side = (threadIdx.x & 31) / GROUP;
+  const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (SIDE * kRows);
+  if (row0 >= p.n_tokens * p.c.heads) return;
+  const Walk first(row0, p.c.heads);
+  int b = seq_of(p.cu, p.n_seqs, first.t);
+  int64_t c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1), base = -1;
+  Held<CODES> kx[kRows], vx[kRows];
+  bool mine[kRows], moved = true, own = false;  // rows that are some sequence's
+  Walk w = first;
+  w.next(side);
+  const Walk begin = w;
+#pragma unroll
+  for (int i = 0; i < kRows; i++) {
+    if (moved) {
+      base = -1;
+      own = false;
+      if (w.t < p.n_tokens) {
+        while (w.t >= c1 && b + 1 < p.n_seqs) b++, c0 = c1, c1 = __ldg(p.cu + b + 1);
+        own = w.t >= c0 && w.t < c1;
+        if (own) base = row_of(p.c, p.table + (int64_t)b * p.ld_table, p.table_width, w.t - c0, 0, p.status);
+      }
+    }
+    mine[i] = own;
+    const int64_t src = base < 0 ? -1 : base + ((int64_t)w.h << p.c.page_log2);
+    load_row<CODES, D>(kx[i], p.c.k, p.c.k_scale, src, lane);
+    load_row<CODES, D>(vx[i], p.c.v, p.c.v_scale, src, lane);
+    moved = w.next(SIDE);
   }
-  *((uint4*)(p.k + t * p.ldk + (int64_t)h * D) + lane) = kx;
-  *((uint4*)(p.v + t * p.ldv + (int64_t)h * D) + lane) = vx;
+  w = begin;
+#pragma unroll
+  for (int i = 0; i < kRows; i++) {
+    if (mine[i]) {
+      uint4* kd = (uint4*)(p.k + w.t * p.ldk + w.h * D) + lane;
+      uint4* vd = (uint4*)(p.v + w.t * p.ldv + w.h * D) + lane;
+#pragma unroll
+      for (int j = 0; j < kHalves; j++) {
+        kd[j * GROUP] = decode_row<CODES>(kx[i], j);
+        vd[j * GROUP] = decode_row<CODES>(vx[i], j);
+      }
+    }
+    w.next(SIDE);
+  }
+}
+
+// Blocks of 8 warps for the rows of n_tokens tokens
+inline int64_t blocks_of(int64_t n_tokens, const mb_kv_cache* c) {
+  const int64_t per_block = 256 / (c->head_dim / 16) * kRows;
+  return (n_tokens * c->n_kv_heads + per_block - 1) / per_block;
 }
 
 // f(codes, head_dim) with both as types
@@ -251,7 +415,7 @@ mb_status mb_kv_write(const mb_kv_cache* cache, const void* k, int64_t ldk, cons
   MB_CHECK(kv_lens, MB_ERR_INVALID, "kv_lens is NULL");
   MB_CHECK(rows_ok(k, ldk, width) && rows_ok(v, ldv, width), MB_ERR_INVALID,
            "k and v must be 16-byte aligned with row strides of at least a row, multiples of 8");
-  const int64_t blocks = (n_tokens * cache->n_kv_heads * (cache->head_dim / 8) + 255) / 256;
+  const int64_t blocks = kv::blocks_of(n_tokens, cache);
   MB_CHECK(blocks < (1LL << 31), MB_ERR_INVALID, "too many rows for one launch");
   MB_CHECK(device_status_ready(), MB_ERR_NOT_READY, "call mb_init on this device first");
   const kv::WriteParams p = {device_cache(cache), (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, ldk, ldv, n_tokens,
@@ -275,7 +439,7 @@ mb_status mb_kv_read(const mb_kv_cache* cache, const int32_t* cu, const int32_t*
   MB_CHECK(cu, MB_ERR_INVALID, "cu is NULL");
   MB_CHECK(rows_ok(k, ldk, width) && rows_ok(v, ldv, width), MB_ERR_INVALID,
            "k and v must be 16-byte aligned with row strides of at least a row, multiples of 8");
-  const int64_t blocks = (n_tokens * cache->n_kv_heads * (cache->head_dim / 8) + 255) / 256;
+  const int64_t blocks = kv::blocks_of(n_tokens, cache);
   MB_CHECK(blocks < (1LL << 31), MB_ERR_INVALID, "too many rows for one launch");
   MB_CHECK(device_status_ready(), MB_ERR_NOT_READY, "call mb_init on this device first");
   const kv::ReadParams p = {device_cache(cache), cu, table, ld_table, table_width, n_seqs, n_tokens,

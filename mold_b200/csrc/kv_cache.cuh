@@ -41,24 +41,6 @@ MB_DEV uint2 ld_stream(const uint2* p) {
   return r;
 }
 
-// The four numbers that a word of 8-bit codes stands for (before the scale), exactly.
-template <int CODES>
-MB_DEV void decode4(uint32_t w, float (&y)[4]) {
-  if (CODES == MB_KV_I8) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) y[j] = (float)(int8_t)(w >> (8 * j));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      uint32_t h;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (16 * j))));
-      const float2 f = __half22float2(*(const __half2*)&h);
-      y[2 * j] = f.x;
-      y[2 * j + 1] = f.y;
-    }
-  }
-}
-
 }  // namespace kv
 
 mb_status check_kv_cache(const mb_kv_cache* c);

@@ -255,6 +255,28 @@ def test_write_odd_rows(cuda, dtype):
     assert (k[:4] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("exponent", [-100, 0, 120])
+def test_write_scales_and_ties(cuda, dtype, exponent):
+    """Rows whose largest value has each of the 128 bf16 fractions, full of values that lie on or next to the border of
+    two codes: scales, inverses and products are rounded as the definition says."""
+    D, half = 128, 0.5 if dtype == torch.int8 else 2.0 ** -4
+    top = torch.arange(128, 256).double() / 128
+    grid = torch.arange(1, D).double() / D
+    codes = torch.floor(grid * 126) + half if dtype == torch.int8 else U.e4m3_values()[torch.arange(1, D) % 119 + 8] * (1 + half)
+    x = torch.cat([top[:, None], codes[None] * top[:, None] / U.TOP[dtype]], 1)
+    x = (x * 2.0 ** exponent).bfloat16()[:, None].cuda()
+    x[:, :, 1::2] *= -1
+    cache, pages = make(dtype, [128], 32, 1, D)
+    cache.write(x, x, pages.table, ints([128]), cu=U.offsets([128]))
+    p, o = pages.rows(0, 128)
+    c, s = U.encode(x, dtype)
+    assert torch.equal(cache.k_scale[p, :, o].cpu(), s) and torch.equal(cache.v_scale[p, :, o].cpu(), s)
+    got = cache.k.view(torch.uint8)[p, :, o]
+    got = got.view(torch.int8).double() if dtype == torch.int8 else U.e4m3_values().cuda()[got.long()]
+    assert torch.equal(got.cpu(), c)
+
+
 def test_write_every_code(cuda):
     """All 256 e4m3 and 255 int8 codes come out of the kernels' decoding as their numbers."""
     t = U.e4m3_values()
