@@ -1,18 +1,24 @@
 // K11: attention of packed prompts, causal or not, grouped heads, on tcgen05 + TMEM (sm_100a).
 //
-// The structure is K4's (attention.cu): two 128-row query tiles a block, scores and output in TMEM, one
-// softmax thread a row, two MMA issuers, 64-key sub-blocks. What differs:
+// One block = one 128-row query tile, two blocks on an SM: while one finds its work, waits for its first
+// tiles or writes its output, the other computes (one block with two tiles, K4's layout, left the tensor
+// pipe at 32 % on a ragged batch).
 //   - A tile's rows are TQ = 128 / G tokens of all G query heads of one key head (row = token * G +
 //     head), one TMA box of G heads x TQ tokens: the group shares each K / V block, and a causal tile
 //     spans few tokens, so little of its diagonal blocks is masked work.
 //   - A block finds its sequence and tile from cu_q by a scan; a sequence's last tiles (the longest under
 //     a causal mask) come first.
-//   - Each tile stops at the last 64-key sub-block that its mask leaves; only sub-blocks that cross a
-//     row's limit are masked.
-//   - Warp 3 guards V: a P V product adds 0 * v for every masked key of a block, so in the blocks that a
-//     mask or the sequence's end crosses it zeroes rows of other sequences and values that are not finite
-//     before the product reads them; rows that may see such a value add it at the end (a slow path that
-//     ordinary data never takes).
+//   warp 0    TMA: the Q tile, then 64-key blocks of K and V into rings of their own.
+//   warp 1    MMA issuer. S(g) = Q K_g^T goes to one half of the S columns while the softmax works on the
+//             other: PV(g), then S(g + 2).
+//   warp 2    guards V: a P V product adds 0 * v for every masked key of a block, so in the blocks that a
+//             mask or the sequence's end crosses it zeroes rows of other sequences and values that are not
+//             finite before the product reads them; rows that may see such a value add it at the end (a
+//             slow path that ordinary data never takes).
+//   warps 4-7 softmax, one thread a query row (= TMEM lane), as in K4 (attention.cu): 64 scores in
+//             registers, P written back over S as bf16, lazy rescale of O, a share of the exponentials on
+//             the FMA pipe. Only blocks that cross a row's limit are masked.
+// TMEM (256 columns a block): S [0, 128) in halves of 64, O [128, 128 + D).
 #include <math.h>
 
 #include <string>
@@ -25,8 +31,9 @@ namespace mb {
 namespace varlen {
 using namespace attn;
 
-constexpr int BKV = 128, NT = 2;
-constexpr int kThreads = 384;
+constexpr int BKV = 64;
+constexpr int kThreads = 256;
+constexpr int kK = 2, kV = 3;  // ring lengths: a V block stays until its P V product, a softmax later
 constexpr float kRescaleThreshold = 8.f;
 constexpr int kPolyPerChunk = 6;  // exponentials of every 32 on the FMA pipe, as in K4
 
@@ -99,33 +106,36 @@ MB_DEV bool find_work(const Params& p, int64_t idx, int span, Work& w) {
 
 template <int D>
 struct Smem {
-  static constexpr uint32_t kTile = 128 * D * 2;
-  static constexpr uint32_t kHalf = 128 * 64 * 2;  // one 64-channel atom column of a tile
-  static constexpr size_t kBytes = 1024 + 6 * (size_t)kTile + 512;
+  static constexpr uint32_t kQ = 128 * D * 2, kQHalf = 128 * 128;        // the Q tile and one 64-channel atom column
+  static constexpr uint32_t kBlock = BKV * D * 2, kHalf = BKV * 128;     // a K or V block
+  static constexpr uint32_t kBars = kQ + (kK + kV) * kBlock;
+  // two blocks on an SM, neither one (shared memory) nor three (TMEM)
+  static constexpr size_t kBytes = kBars + 512 < 80 * 1024 ? 80 * 1024 : kBars + 512;
+  static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two blocks on an SM");
 };
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 2)
     k_attention_varlen(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                        const __grid_constant__ CUtensorMap tv, const Params p) {
-  constexpr uint32_t kTile = Smem<D>::kTile, kHalf = Smem<D>::kHalf;
+  using S = Smem<D>;
   constexpr int CH = D / 64;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t* sQ = smem;              // 2 tiles
-  uint8_t* sK = smem + 2 * kTile;  // 2 stages
-  uint8_t* sV = smem + 4 * kTile;  // 2 stages
-  uint64_t* bars = (uint64_t*)(smem + 6 * kTile);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + S::kQ;
+  uint8_t* sV = sK + kK * S::kBlock;
+  uint64_t* bars = (uint64_t*)(smem + S::kBars);
   uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;    // [2] per stage
-  uint64_t* v_full = bars + 3;    // [2]
-  uint64_t* kv_empty = bars + 5;  // [2]
-  uint64_t* s_full = bars + 7;    // [tile][half]
-  uint64_t* p_full = bars + 11;   // [tile][half]
-  uint64_t* o_full = bars + 15;   // [tile]
-  uint64_t* pv_done = bars + 17;  // [tile]
-  uint64_t* v_ok = bars + 19;     // [2] per stage: guarded blocks
-  uint32_t* tmem_slot = (uint32_t*)(bars + 21);
+  uint64_t* k_full = bars + 1;    // [kK]
+  uint64_t* k_empty = bars + 3;   // [kK]
+  uint64_t* v_full = bars + 5;    // [kV]
+  uint64_t* v_ok = bars + 8;      // [kV]: guarded blocks
+  uint64_t* v_empty = bars + 11;  // [kV]
+  uint64_t* s_full = bars + 14;   // [half]
+  uint64_t* p_full = bars + 16;   // [half]
+  uint64_t* o_full = bars + 18;
+  uint64_t* pv_done = bars + 19;  // one completion per P V product
+  uint32_t* tmem_slot = (uint32_t*)(bars + 20);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* odd_v = (volatile int*)(tmem_slot + 2);  // a value that is not finite was zeroed
   int* found = (int*)(tmem_slot + 3);
@@ -138,23 +148,26 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     Work w;
-    const bool ok = find_work(p, item, NT * TQ, w);
+    const bool ok = find_work(p, item, TQ, w);
     if (lane == 0) {
       *found = ok;
       if (ok) *work = w;
       mbar_init(q_full, 1);
-      for (int i = 0; i < 2; i++) {
+      for (int i = 0; i < kK; i++) {
         mbar_init(&k_full[i], 1);
+        mbar_init(&k_empty[i], 1);
+      }
+      for (int i = 0; i < kV; i++) {
         mbar_init(&v_full[i], 1);
         mbar_init(&v_ok[i], 1);
-        mbar_init(&kv_empty[i], 3);  // one arrival per MMA issuer and one of the V guard
-        mbar_init(&o_full[i], 1);
-        mbar_init(&pv_done[i], 1);
+        mbar_init(&v_empty[i], 2);  // the MMA issuer's and the guard's
       }
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < 2; i++) {
         mbar_init(&s_full[i], 1);
         mbar_init(&p_full[i], 4);
       }
+      mbar_init(o_full, 1);
+      mbar_init(pv_done, 1);
       *abort_flag = 0;
       *odd_v = 0;
       fence_mbar_init();
@@ -163,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (!*found) return;
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -174,191 +187,156 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // keys that the mask leaves token i of the sequence: the first keys_of(i)
   auto keys_of = [&](int i) { return p.causal ? max(0, min(i + 1 + w.n - w.m, w.n)) : w.n; };
-  // sub-blocks of tile t, and the keys that all of its rows see
-  auto tile_subs = [&](int t) {
-    const int first = w.tok0 + t * TQ;
-    return first >= w.m ? 0 : (keys_of(min(first + TQ, w.m) - 1) + 63) / 64;
-  };
-  const int n_sub0 = tile_subs(0), n_sub1 = tile_subs(1);
-  const int n_kv = (max(n_sub0, n_sub1) + 1) / 2;
+  const int all_see = keys_of(w.tok0);  // keys that every row sees
+  const int n_kv = (keys_of(min(w.tok0 + TQ, w.m) - 1) + BKV - 1) / BKV;
   // blocks from this one on hold keys that some row is not to see
-  const int guard0 = keys_of(w.tok0) / BKV;
+  const int guard0 = all_see / BKV;
 
   if (warp == 0) {
     if (lane == 0 && n_kv > 0) {
       tma_prefetch_desc(&tq);
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
-      const int tiles = n_sub1 > 0 ? 2 : 1;  // tile 1 never has fewer keys than tile 0
-      mbar_expect_tx(q_full, (uint32_t)(tiles * CH * G * TQ * 128));
-      for (int t = 0; t < tiles; t++)
-        for (int c = 0; c < CH; c++)
-          tma_load_3d(sQ + t * kTile + c * kHalf, &tq, q_full, c * 64, hk * G, w.q_start + w.tok0 + t * TQ);
-      for (int j = 0; j < n_kv; j++) {
-        const int s = j & 1;
-        const uint32_t ph = (j >> 1) & 1;
-        if (!(mbar_wait(&kv_empty[s], ph ^ 1, abort_flag, p.status, kDevTimeoutAttn))) break;
-        mbar_expect_tx(&k_full[s], kTile);
-        for (int c = 0; c < CH; c++)
-          tma_load_3d(sK + s * kTile + c * kHalf, &tk, &k_full[s], c * 64, hk, w.k_start + j * BKV);
-        mbar_expect_tx(&v_full[s], kTile);
-        for (int c = 0; c < CH; c++)
-          tma_load_3d(sV + s * kTile + c * kHalf, &tv, &v_full[s], c * 64, hk, w.k_start + j * BKV);
+      mbar_expect_tx(q_full, (uint32_t)(CH * G * TQ * 128));
+      for (int c = 0; c < CH; c++)
+        tma_load_3d(sQ + c * S::kQHalf, &tq, q_full, c * 64, hk * G, w.q_start + w.tok0);
+      // V of block j - 1 after K of block j: the scores need their K first
+      for (int j = 0; j <= n_kv; j++) {
+        if (j < n_kv) {
+          const int s = j % kK;
+          if (!mbar_wait(&k_empty[s], ((j / kK) & 1) ^ 1, abort_flag, p.status, kDevTimeoutAttn)) break;
+          mbar_expect_tx(&k_full[s], S::kBlock);
+          for (int c = 0; c < CH; c++)
+            tma_load_3d(sK + s * S::kBlock + c * S::kHalf, &tk, &k_full[s], c * 64, hk, w.k_start + j * BKV);
+        }
+        if (j > 0) {
+          const int i = j - 1, s = i % kV;
+          if (!mbar_wait(&v_empty[s], ((i / kV) & 1) ^ 1, abort_flag, p.status, kDevTimeoutAttn)) break;
+          mbar_expect_tx(&v_full[s], S::kBlock);
+          for (int c = 0; c < CH; c++)
+            tma_load_3d(sV + s * S::kBlock + c * S::kHalf, &tv, &v_full[s], c * 64, hk, w.k_start + i * BKV);
+        }
       }
     }
-  } else if (warp == 1 || warp == 2) {
-    const int t = warp - 1;
-    constexpr uint32_t idesc_s = idesc_bf16(128, 64, false);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = idesc_bf16(128, BKV, false);
     constexpr uint32_t idesc_o = idesc_bf16(128, D, true);
-    const uint32_t qa = smem_u32(sQ) + t * kTile;
-    const int n_sub = t ? n_sub1 : n_sub0;
-    bool ok = n_kv == 0 || mbar_wait(q_full, 0, abort_flag, p.status, kDevTimeoutAttn);
-    // S_t(g) = Q_t K_g^T (64 keys) into S half g & 1
+    const uint32_t qa = smem_u32(sQ);
+    bool ok = n_kv > 0 && mbar_wait(q_full, 0, abort_flag, p.status, kDevTimeoutAttn);
+    // S(g) = Q K_g^T into S half g & 1
     auto issue_s = [&](int g) {
-      const int hh = g & 1;
-      const uint32_t ka = smem_u32(sK + ((g >> 1) & 1) * kTile) + hh * 8192;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; kk++) {
-        const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
-        umma_ss_elect(tmem + t * 128 + hh * 64, sw128_desc(qa + off, 16, 1024), sw128_desc(ka + off, 16, 1024),
-                      idesc_s, kk > 0);
-      }
-      if (lane == 0) umma_commit(&s_full[t * 2 + hh]);
-      __syncwarp();
-    };
-    // O_t += P_t(g) V_g; the block's stage is released with the tile's last sub-block of it
-    auto issue_pv = [&](int g) {
-      const int hh = g & 1;
-      const uint32_t va = smem_u32(sV + ((g >> 1) & 1) * kTile);
-#pragma unroll
-      for (int kk = 0; kk < 4; kk++) {
-        const uint64_t bdesc = sw128_desc(va + (hh * 4 + kk) * 16 * 128, kHalf, 1024);
-        umma_ts_elect(tmem + 256 + t * 128, tmem + t * 128 + hh * 64 + kk * 8, bdesc, idesc_o,
-                      (g > 0 || kk > 0) ? 1u : 0u);
-      }
-      if (lane == 0) {
-        umma_commit(&pv_done[t]);
-        if (hh == 1 || g == n_sub - 1) umma_commit(&kv_empty[(g >> 1) & 1]);
-      }
-      __syncwarp();
-    };
-    if (ok && n_sub > 0) {
-      if ((ok = mbar_wait(&k_full[0], 0, abort_flag, p.status, kDevTimeoutAttn))) {
-        tc_fence_after();
-        issue_s(0);
-        if (n_sub > 1) issue_s(1);
-      }
-    }
-    for (int g = 0; g < n_sub && ok; g++) {
-      const int hh = g & 1, j = g >> 1;
-      if (hh == 0) {
-        if (!(ok = j < guard0 ? mbar_wait(&v_full[j & 1], (j >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn)
-                              : mbar_wait(&v_ok[j & 1], ((j - guard0) >> 1) & 1, abort_flag, p.status,
-                                          kDevTimeoutAttn)))
-          break;
-      }
-      if (!(ok = (mbar_wait(&p_full[t * 2 + hh], j & 1, abort_flag, p.status, kDevTimeoutAttn)))) break;
+      const int s = g % kK;
+      if (!(ok = mbar_wait(&k_full[s], (g / kK) & 1, abort_flag, p.status, kDevTimeoutAttn))) return;
       tc_fence_after();
-      issue_pv(g);
-      if (g + 2 < n_sub) {
-        if (hh == 0 &&
-            !(ok = (mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))))
-          break;
-        tc_fence_after();
-        issue_s(g + 2);
+      const uint32_t ka = smem_u32(sK) + s * S::kBlock;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk++)
+        umma_ss_elect(tmem + (g & 1) * 64, sw128_desc(qa + (kk >> 2) * S::kQHalf + (kk & 3) * 32, 16, 1024),
+                      sw128_desc(ka + (kk >> 2) * S::kHalf + (kk & 3) * 32, 16, 1024), idesc_s, kk > 0);
+      if (lane == 0) {
+        umma_commit(&s_full[g & 1]);
+        umma_commit(&k_empty[s]);
       }
-    }
-    if (ok && n_sub > 0 && lane == 0) umma_commit(&o_full[t]);
-    __syncwarp();
-    // blocks that only the other tile reads: this issuer's arrival once each has been loaded
-    for (int j = (n_sub + 1) / 2; j < n_kv && ok; j++) {
-      ok = mbar_wait(&k_full[j & 1], (j >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn);
-      if (ok && lane == 0) mbar_arrive(&kv_empty[j & 1]);
       __syncwarp();
+    };
+    if (ok) issue_s(0);
+    if (ok && n_kv > 1) issue_s(1);
+    for (int g = 0; g < n_kv && ok; g++) {
+      const int s = g % kV;
+      if (!(ok = g < guard0
+                     ? mbar_wait(&v_full[s], (g / kV) & 1, abort_flag, p.status, kDevTimeoutAttn)
+                     : mbar_wait(&v_ok[s], ((g - guard0) / kV) & 1, abort_flag, p.status, kDevTimeoutAttn)))
+        break;
+      if (!(ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
+      tc_fence_after();
+      // O += P(g) V_g, P read from TMEM (bf16 pairs over the first 32 columns of its S half); V [keys, d] is MN-major:
+      // 64-wide d chunks kHalf apart, 8-key groups 1024 B apart
+      const uint32_t va = smem_u32(sV) + s * S::kBlock;
+#pragma unroll
+      for (int kk = 0; kk < BKV / 16; kk++)
+        umma_ts_elect(tmem + 128, tmem + (g & 1) * 64 + kk * 8, sw128_desc(va + kk * 16 * 128, S::kHalf, 1024), idesc_o,
+                      (g > 0 || kk > 0) ? 1u : 0u);
+      if (lane == 0) {
+        umma_commit(pv_done);
+        umma_commit(&v_empty[s]);
+      }
+      __syncwarp();
+      if (g + 2 < n_kv) issue_s(g + 2);
     }
-  } else if (warp == 3) {
+    if (ok && lane == 0) umma_commit(o_full);
+    __syncwarp();
+  } else if (warp == 2) {
     // ---------------------------------------------------------------- V guard
     // Takes part in every block, so that it never falls a phase of a barrier behind.
     for (int j = 0; j < n_kv; j++) {
-      const int s = j & 1;
-      if (!mbar_wait(&v_full[s], (j >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn)) break;
-      if (j < guard0) {
-        if (lane == 0) mbar_arrive(&kv_empty[s]);
-        __syncwarp();
-        continue;
-      }
-      uint8_t* v = sV + s * kTile;
-      // 16-byte pieces by address: a row is 128 bytes of each atom column, and the swizzle moves pieces
-      // inside a row only
-      const int rows = min(BKV, w.n - j * BKV);
-      for (int i = rows * 8 + lane; i < BKV * 8; i += 32)
+      const int s = j % kV;
+      if (!mbar_wait(&v_full[s], (j / kV) & 1, abort_flag, p.status, kDevTimeoutAttn)) break;
+      if (j >= guard0) {
+        uint8_t* v = sV + s * S::kBlock;
+        // 16-byte pieces by address: a row is 128 bytes of each atom column, and the swizzle moves pieces
+        // inside a row only
+        const int rows = min(BKV, w.n - j * BKV);
+        for (int i = rows * 8 + lane; i < BKV * 8; i += 32)
 #pragma unroll
-        for (int c = 0; c < CH; c++) *(uint4*)(v + c * kHalf + i * 16) = make_uint4(0, 0, 0, 0);
-      if (p.causal) {
-        __nv_bfloat162 acc = __float2bfloat162_rn(0.f);
-        const __nv_bfloat162 zero = acc;
-        for (int c = 0; c < CH; c++)
-#pragma unroll 4
-          for (int i = lane; i < rows * 8; i += 32) {
-            const uint4 x = *(const uint4*)(v + c * kHalf + i * 16);
-            acc = __hfma2(*(const __nv_bfloat162*)&x.x, zero, acc);  // NaN from what is not finite, and it stays
-            acc = __hfma2(*(const __nv_bfloat162*)&x.y, zero, acc);
-            acc = __hfma2(*(const __nv_bfloat162*)&x.z, zero, acc);
-            acc = __hfma2(*(const __nv_bfloat162*)&x.w, zero, acc);
-          }
-        const uint32_t bits = *(const uint32_t*)&acc;
-        if (!finite_bf16(bits) || !finite_bf16(bits >> 16)) {
-          *odd_v = 1;
+          for (int c = 0; c < CH; c++) *(uint4*)(v + c * S::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+        if (p.causal) {
+          __nv_bfloat162 acc = __float2bfloat162_rn(0.f);
+          const __nv_bfloat162 zero = acc;
           for (int c = 0; c < CH; c++)
+#pragma unroll 4
             for (int i = lane; i < rows * 8; i += 32) {
-              uint32_t* x = (uint32_t*)(v + c * kHalf + i * 16);
-              for (int e = 0; e < 4; e++) {
-                uint32_t y = x[e];
-                if (!finite_bf16(y)) y &= 0xffff0000u;
-                if (!finite_bf16(y >> 16)) y &= 0x0000ffffu;
-                x[e] = y;
-              }
+              const uint4 x = *(const uint4*)(v + c * S::kHalf + i * 16);
+              acc = __hfma2(*(const __nv_bfloat162*)&x.x, zero, acc);  // NaN from what is not finite, and it stays
+              acc = __hfma2(*(const __nv_bfloat162*)&x.y, zero, acc);
+              acc = __hfma2(*(const __nv_bfloat162*)&x.z, zero, acc);
+              acc = __hfma2(*(const __nv_bfloat162*)&x.w, zero, acc);
             }
+          const uint32_t bits = *(const uint32_t*)&acc;
+          if (!finite_bf16(bits) || !finite_bf16(bits >> 16)) {
+            *odd_v = 1;
+            for (int c = 0; c < CH; c++)
+              for (int i = lane; i < rows * 8; i += 32) {
+                uint32_t* x = (uint32_t*)(v + c * S::kHalf + i * 16);
+                for (int e = 0; e < 4; e++) {
+                  uint32_t y = x[e];
+                  if (!finite_bf16(y)) y &= 0xffff0000u;
+                  if (!finite_bf16(y >> 16)) y &= 0x0000ffffu;
+                  x[e] = y;
+                }
+              }
+          }
         }
+        fence_proxy_async_smem();
       }
-      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&v_ok[s]);
-        mbar_arrive(&kv_empty[s]);
+        if (j >= guard0) mbar_arrive(&v_ok[s]);
+        mbar_arrive(&v_empty[s]);
       }
       __syncwarp();
     }
-  } else {
+  } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax
-    // 4 warps per tile; thread = query row = TMEM lane.
-    const int t = (warp - 4) >> 2;
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;
-    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + t * 128 + lane_addr, tO = tmem + 256 + t * 128 + lane_addr;
-    const int first = w.tok0 + t * TQ;
-    const int tok = first + r / G, head = hk * G + r % G;
+    const int r = (warp - 4) * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)((warp - 4) * 32) << 16;
+    const uint32_t tO = tmem + 128 + lane_addr;
+    const int tok = w.tok0 + r / G, head = hk * G + r % G;
     const bool mine = r < TQ * G && tok < w.m;  // this row is one of the sequence's
     const int keys = keys_of(min(tok, w.m - 1));
-    const int all_see = keys_of(min(first, w.m - 1));
-    const int n_sub = t ? n_sub1 : n_sub0;
     const float sc = p.scale_log2;
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
-    for (int g = 0; g < n_sub; g++) {
-      const int hh = g & 1;
-      if (!(ok = (mbar_wait(&s_full[t * 2 + hh], (g >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))))
-        break;
+    for (int g = 0; g < n_kv; g++) {
+      if (!(ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
       tc_fence_after();
-      const uint32_t tSh = tS + hh * 64;
+      const uint32_t tSh = tmem + (g & 1) * 64 + lane_addr;
       uint32_t v[2][32];
       tmem_ld32(tSh, v[0]);
       tmem_ld32(tSh + 32, v[1]);
       tmem_wait_ld();
-      const bool masked = (g + 1) * 64 > all_see;  // the same for the whole tile
+      const bool masked = (g + 1) * BKV > all_see;  // the same for the whole tile
       if (masked) {
-        const int valid = keys - g * 64;
+        const int valid = keys - g * BKV;
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
@@ -380,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float ref = m_run == -INFINITY ? 0.f : m_run;  // no key so far: weights 0
       const uint64_t sc2 = pk2(sc, sc), nm2 = pk2(-ref, -ref);
       uint64_t sum2 = pk2(0.f, 0.f);
-      // In masked sub-blocks all exponentials are the exact-zero kind: the polynomial ends at 2^-126.
+      // In masked blocks all exponentials are the exact-zero kind: the polynomial ends at 2^-126.
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         uint32_t pk[16];
@@ -404,8 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float sa, sb;
       up2(sum2, sa, sb);
       if (g > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        // O_t must hold P V of sub-block g - 1 before it is rescaled
-        if (!(ok = mbar_wait(&pv_done[t], (g - 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
+        // O must hold P V of block g - 1 before it is rescaled
+        if (!(ok = mbar_wait(pv_done, (g - 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D / 32; c++) {
@@ -421,9 +399,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       l_run = l_run * alpha + (sa + sb);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t * 2 + hh]);
+      if (lane == 0) mbar_arrive(&p_full[g & 1]);
     }
-    if (ok && n_sub > 0) ok = mbar_wait(&o_full[t], 0, abort_flag, p.status, kDevTimeoutAttn);
+    if (ok && n_kv > 0) ok = mbar_wait(o_full, 0, abort_flag, p.status, kDevTimeoutAttn);
     if (ok) {
       tc_fence_after();
       // a row without keys is 0; a maximum of NaN or +inf, or -inf over keys, makes softmax NaN
@@ -433,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < D / 32; c++) {
         uint32_t o[32];
-        if (n_sub > 0) {
+        if (n_kv > 0) {
           tmem_ld32(tO + c * 32, o);
           tmem_wait_ld();
         }
@@ -471,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -496,7 +474,7 @@ cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, i
     if (e != cudaSuccess) return e;
     attr_done[dev & 63] = 1;
   }
-  const int64_t blocks = (p.total_q / (NT * p.TQ) + p.n_seqs) * p.Hkv;  // each sequence rounds up once
+  const int64_t blocks = (p.total_q / p.TQ + p.n_seqs) * p.Hkv;  // each sequence rounds up once
   if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
   k_attention_varlen<D><<<(unsigned)blocks, kThreads, Smem<D>::kBytes, st>>>(tq, tk, tv, p);
   return cudaGetLastError();
