@@ -16,8 +16,8 @@
 //             finite before the product reads them; rows that may see such a value add it at the end (a
 //             slow path that ordinary data never takes).
 //   warps 4-7 softmax, one thread a query row (= TMEM lane), as in K4 (attention.cu): 64 scores in
-//             registers, P written back over S as bf16, lazy rescale of O, a share of the exponentials on
-//             the FMA pipe. Only blocks that cross a row's limit are masked.
+//             registers, P written back over S as bf16, lazy rescale of O. Only blocks that cross a row's
+//             limit are masked.
 // TMEM (256 columns a block): S [0, 128) in halves of 64, O [128, 128 + D).
 #include <math.h>
 
@@ -35,7 +35,6 @@ constexpr int BKV = 64;
 constexpr int kThreads = 256;
 constexpr int kK = 2, kV = 3;  // ring lengths: a V block stays until its P V product, a softmax later
 constexpr float kRescaleThreshold = 8.f;
-constexpr int kPolyPerChunk = 6;  // exponentials of every 32 on the FMA pipe, as in K4
 
 struct Params {
   const int32_t *cu_q, *cu_k;
@@ -76,10 +75,12 @@ MB_DEV bool find_work(const Params& p, int64_t idx, int span, Work& w) {
   auto clampk = [&](int64_t x) { return (int)(x < 0 ? 0 : x < p.total_k ? x : p.total_k); };
   for (int base = 0; base < p.n_seqs; base += 32) {
     const int b = base + lane;
-    int q0 = 0, m = 0;
+    int q0 = 0, m = 0, k0 = 0, n = 0;
     if (b < p.n_seqs) {
       q0 = clampq(__ldg(p.cu_q + b));
       m = max(0, clampq(__ldg(p.cu_q + b + 1)) - q0);
+      k0 = clampk(__ldg(p.cu_k + b));
+      n = max(0, clampk(__ldg(p.cu_k + b + 1)) - k0);
     }
     int64_t x = (m + span - 1) / span;
 #pragma unroll
@@ -93,9 +94,8 @@ MB_DEV bool find_work(const Params& p, int64_t idx, int span, Work& w) {
       const int64_t end = __shfl_sync(0xffffffffu, x, src);
       w.q_start = __shfl_sync(0xffffffffu, q0, src);
       w.m = __shfl_sync(0xffffffffu, m, src);
-      const int k0 = clampk(__ldg(p.cu_k + base + src));
-      w.k_start = k0;
-      w.n = max(0, clampk(__ldg(p.cu_k + base + src + 1)) - k0);
+      w.k_start = __shfl_sync(0xffffffffu, k0, src);
+      w.n = __shfl_sync(0xffffffffu, n, src);
       w.tok0 = (int)(end - 1 - idx) * span;  // last tile first
       return true;
     }
@@ -117,7 +117,7 @@ struct Smem {
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2)
     k_attention_varlen(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                       const __grid_constant__ CUtensorMap tv, const Params p) {
+                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to, const Params p) {
   using S = Smem<D>;
   constexpr int CH = D / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -173,8 +173,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       fence_mbar_init();
     }
   }
-  __syncthreads();
-  if (!*found) return;
   if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
@@ -183,6 +181,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (!*found) {
+    if (warp == 1) tmem_dealloc(tmem, 256);
+    return;
+  }
   const Work w = *work;
 
   // keys that the mask leaves token i of the sequence: the first keys_of(i)
@@ -325,9 +327,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int keys = keys_of(min(tok, w.m - 1));
     const float sc = p.scale_log2;
     float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true;
+    bool ok = true, ready = false;
     for (int g = 0; g < n_kv; g++) {
-      if (!(ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
+      if (!ready && !(ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
       tc_fence_after();
       const uint32_t tSh = tmem + (g & 1) * 64 + lane_addr;
       uint32_t v[2][32];
@@ -343,14 +345,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < 32; i++)
             if (c * 32 + i >= valid) v[c][i] = __float_as_uint(-INFINITY);
       }
-      float mc[2];
+      float mc[4];  // four independent chains
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        mc[c] = max_nan(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
+      for (int c = 0; c < 4; c++) {
+        const uint32_t* x = &v[c >> 1][(c & 1) * 16];
+        mc[c] = max_nan(__uint_as_float(x[0]), __uint_as_float(x[1]));
 #pragma unroll
-        for (int i = 2; i < 32; i += 2) mc[c] = max3_nan(mc[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+        for (int i = 2; i < 16; i += 2) mc[c] = max3_nan(mc[c], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
       }
-      const float m_new = max_nan(m_run, max_nan(mc[0], mc[1]) * sc);
+      const float m_new = max_nan(m_run, max3_nan(mc[0], mc[1], max_nan(mc[2], mc[3])) * sc);
       // lazy rescale: only rows whose max grew by more than 2^8 (or turned NaN) move their reference point
       const bool need = g == 0 || !(m_new <= m_run + kRescaleThreshold);
       const float alpha = (need && g > 0 && mine) ? ex2_approx(m_run - m_new) : 1.f;
@@ -358,22 +361,17 @@ __global__ void __launch_bounds__(kThreads, 2)
       const float ref = m_run == -INFINITY ? 0.f : m_run;  // no key so far: weights 0
       const uint64_t sc2 = pk2(sc, sc), nm2 = pk2(-ref, -ref);
       uint64_t sum2 = pk2(0.f, 0.f);
-      // In masked blocks all exponentials are the exact-zero kind: the polynomial ends at 2^-126.
+      // All exponentials on the MUFU pipe: with K4's share of 6 in 32 as polynomials on the FMA pipe this kernel lost 10 %
+      // (8201 tokens, 32/8 heads: 556 -> 618 us).
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         uint32_t pk[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const uint64_t x2 = fma2(pk2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sc2, nm2);
-          float e0, e1;
-          if (2 * i < kPolyPerChunk && !masked) {
-            exp2_poly3(x2, e0, e1);
-          } else {
-            float x0, x1;
-            up2(x2, x0, x1);
-            e0 = ex2_approx(x0);
-            e1 = ex2_approx(x1);
-          }
+          float x0, x1;
+          up2(x2, x0, x1);
+          const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
           sum2 = add2(sum2, pk2(e0, e1));
           pk[i] = pack_bf16x2(e0, e1);
         }
@@ -395,6 +393,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           tmem_st32(tO + c * 32, o);
         }
       }
+      // the next scores are usually there: ask while the stores are on their way
+      ready = g + 1 < n_kv && mbar_try_wait(&s_full[(g + 1) & 1], ((g + 1) >> 1) & 1);
       tmem_wait_st();
       l_run = l_run * alpha + (sa + sb);
       tc_fence_before();
@@ -402,6 +402,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (lane == 0) mbar_arrive(&p_full[g & 1]);
     }
     if (ok && n_kv > 0) ok = mbar_wait(o_full, 0, abort_flag, p.status, kDevTimeoutAttn);
+    // A tile whose tokens all belong to the sequence is gathered in the Q tile's place (its last product is done) and
+    // stored by TMA, row by row by its threads otherwise (4400 cycles for every tile when all were).
+    const bool whole = w.tok0 + TQ <= w.m;
     if (ok) {
       tc_fence_after();
       // a row without keys is 0; a maximum of NaN or +inf, or -inf over keys, makes softmax NaN
@@ -430,17 +433,28 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
           }
         }
-        if (mine) {
 #pragma unroll
-          for (int u = 0; u < 4; u++) {
-            uint4 w4;
-            w4.x = pack_bf16x2(__uint_as_float(o[8 * u + 0]), __uint_as_float(o[8 * u + 1]));
-            w4.y = pack_bf16x2(__uint_as_float(o[8 * u + 2]), __uint_as_float(o[8 * u + 3]));
-            w4.z = pack_bf16x2(__uint_as_float(o[8 * u + 4]), __uint_as_float(o[8 * u + 5]));
-            w4.w = pack_bf16x2(__uint_as_float(o[8 * u + 6]), __uint_as_float(o[8 * u + 7]));
+        for (int u = 0; u < 4; u++) {
+          uint4 w4;
+          w4.x = pack_bf16x2(__uint_as_float(o[8 * u + 0]), __uint_as_float(o[8 * u + 1]));
+          w4.y = pack_bf16x2(__uint_as_float(o[8 * u + 2]), __uint_as_float(o[8 * u + 3]));
+          w4.z = pack_bf16x2(__uint_as_float(o[8 * u + 4]), __uint_as_float(o[8 * u + 5]));
+          w4.w = pack_bf16x2(__uint_as_float(o[8 * u + 6]), __uint_as_float(o[8 * u + 7]));
+          if (whole)
+            *(uint4*)(sQ + (c >> 1) * S::kQHalf + r * 128 + ((((c & 1) * 4 + u) ^ (r & 7)) << 4)) = w4;
+          else if (mine)
             *(uint4*)(orow + c * 32 + u * 8) = w4;
-          }
         }
+      }
+    }
+    if (whole) {
+      fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // the softmax warps, which all come here
+      if (warp == 4 && lane == 0 && ok) {
+        for (int c = 0; c < CH; c++)
+          tma_store_3d(&to, sQ + c * S::kQHalf, c * 64, hk * G, w.q_start + w.tok0);
+        bulk_commit();
+        bulk_wait_read();
       }
     }
   }
@@ -455,11 +469,13 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 template <int D>
 cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, int64_t ldk, int H, cudaStream_t st) {
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   const uint64_t head = D * 2, keys = p.total_k > 0 ? (uint64_t)p.total_k : 1;
   // {channel, head, token}; a sequence's end inside a box reads the next sequence's rows, which the masks leave out
   if (!make_tmap_3d(&tq, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)H, (uint64_t)p.total_q, head,
                     (uint64_t)ldq * 2, 64, (uint32_t)p.G, (uint32_t)p.TQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tmap_3d(&to, p.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)H, (uint64_t)p.total_q, head,
+                    (uint64_t)p.ldo * 2, 64, (uint32_t)p.G, (uint32_t)p.TQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tmap_3d(&tk, k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)p.Hkv, keys, head,
                     (uint64_t)ldk * 2, 64, 1, BKV, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tmap_3d(&tv, p.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)p.Hkv, keys, head,
@@ -476,7 +492,7 @@ cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, i
   }
   const int64_t blocks = (p.total_q / p.TQ + p.n_seqs) * p.Hkv;  // each sequence rounds up once
   if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  k_attention_varlen<D><<<(unsigned)blocks, kThreads, Smem<D>::kBytes, st>>>(tq, tk, tv, p);
+  k_attention_varlen<D><<<(unsigned)blocks, kThreads, Smem<D>::kBytes, st>>>(tq, tk, tv, to, p);
   return cudaGetLastError();
 }
 
