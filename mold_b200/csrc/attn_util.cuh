@@ -79,5 +79,37 @@ MB_DEV void umma_ts_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint
       : "memory");
 }
 
+// Four products in a row under one election: depth steps of 16 that lie 32 bytes apart in both operands (64 elements of
+// one 128-byte swizzle atom column, K-major).
+MB_DEV void umma_ss_x4_elect(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b32 r;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, %3, %3;\n"
+      " elect.sync r|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      " add.s64 a, %1, 2;\n add.s64 b, %2, 2;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 4;\n add.s64 b, %2, 4;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n"
+      " add.s64 a, %1, 6;\n add.s64 b, %2, 6;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in TMEM (8 columns a step) and B MN-major: 16 rows of 128 bytes a step.
+MB_DEV void umma_ts_x4_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, t, e;\n .reg .b32 r, a;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, %3, %3;\n"
+      " elect.sync r|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " add.s32 a, %1, 8;\n add.s64 b, %2, 128;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+      " add.s32 a, %1, 16;\n add.s64 b, %2, 256;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n"
+      " add.s32 a, %1, 24;\n add.s64 b, %2, 384;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 }  // namespace attn
 }  // namespace mb

@@ -232,9 +232,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       tc_fence_after();
       const uint32_t ka = smem_u32(sK) + s * S::kBlock;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; kk++)
-        umma_ss_elect(tmem + (g & 1) * 64, sw128_desc(qa + (kk >> 2) * S::kQHalf + (kk & 3) * 32, 16, 1024),
-                      sw128_desc(ka + (kk >> 2) * S::kHalf + (kk & 3) * 32, 16, 1024), idesc_s, kk > 0);
+      for (int c = 0; c < CH; c++)
+        umma_ss_x4_elect(tmem + (g & 1) * 64, sw128_desc(qa + c * S::kQHalf, 16, 1024),
+                         sw128_desc(ka + c * S::kHalf, 16, 1024), idesc_s, c > 0);
       if (lane == 0) {
         umma_commit(&s_full[g & 1]);
         umma_commit(&k_empty[s]);
@@ -254,10 +254,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       // O += P(g) V_g, P read from TMEM (bf16 pairs over the first 32 columns of its S half); V [keys, d] is MN-major:
       // 64-wide d chunks kHalf apart, 8-key groups 1024 B apart
       const uint32_t va = smem_u32(sV) + s * S::kBlock;
-#pragma unroll
-      for (int kk = 0; kk < BKV / 16; kk++)
-        umma_ts_elect(tmem + 128, tmem + (g & 1) * 64 + kk * 8, sw128_desc(va + kk * 16 * 128, S::kHalf, 1024), idesc_o,
-                      (g > 0 || kk > 0) ? 1u : 0u);
+      umma_ts_x4_elect(tmem + 128, tmem + (g & 1) * 64, sw128_desc(va, S::kHalf, 1024), idesc_o, g > 0 ? 1u : 0u);
       if (lane == 0) {
         umma_commit(pv_done);
         umma_commit(&v_empty[s]);
