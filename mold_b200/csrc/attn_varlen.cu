@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int c = 0; c < CH; c++)
         tma_load_3d(sQ + c * S::kQHalf, &tq, q_full, c * 64, hk * G, w.q_start + w.tok0);
       // V of block j - 1 after K of block j: the scores need their K first
+      int nk = 0, nv = 0;
       for (int j = 0; j <= n_kv; j++) {
         if (j < n_kv) {
           const int s = j % kK;
@@ -210,6 +211,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           mbar_expect_tx(&k_full[s], S::kBlock);
           for (int c = 0; c < CH; c++)
             tma_load_3d(sK + s * S::kBlock + c * S::kHalf, &tk, &k_full[s], c * 64, hk, w.k_start + j * BKV);
+          nk++;
         }
         if (j > 0) {
           const int i = j - 1, s = i % kV;
@@ -217,8 +219,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           mbar_expect_tx(&v_full[s], S::kBlock);
           for (int c = 0; c < CH; c++)
             tma_load_3d(sV + s * S::kBlock + c * S::kHalf, &tv, &v_full[s], c * 64, hk, w.k_start + i * BKV);
+          nv++;
         }
       }
+      // the block's memory must outlive its copies, whatever the other warps do
+      volatile int never = 0;
+      mbar_wait(q_full, 0, &never, p.status, kDevTimeoutAttn);
+      for (int j = max(nk - kK, 0); j < nk; j++)
+        mbar_wait(&k_full[j % kK], (j / kK) & 1, &never, p.status, kDevTimeoutAttn);
+      for (int j = max(nv - kV, 0); j < nv; j++)
+        mbar_wait(&v_full[j % kV], (j / kV) & 1, &never, p.status, kDevTimeoutAttn);
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = idesc_bf16(128, BKV, false);
