@@ -387,7 +387,7 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
 def _out(out, q):
     """(out, address, row stride): the caller's tensor, or a new one, shaped like q."""
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         return out, out.data_ptr(), q.shape[1] * q.shape[2]
     if out.shape != q.shape:
         raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
@@ -485,7 +485,7 @@ class KVCache:
             n_tokens = int(cu[-1]) if n_tokens is None else int(n_tokens)
             shape = (n_tokens, self.n_kv_heads, self.head_dim)
             k = torch.empty(shape, dtype=torch.bfloat16, device=self.k.device)
-            v = torch.empty(shape, dtype=torch.bfloat16, device=self.k.device)
+            v = torch.empty_like(k)
         k, k_ptr, ldk, rows = self._rows(k, "k", copy=False)
         v, v_ptr, ldv, v_rows = self._rows(v, "v", copy=False)
         if rows != v_rows or (n_tokens is not None and n_tokens != rows):
