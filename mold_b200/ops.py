@@ -484,7 +484,7 @@ class KVCache:
         if k is None:
             n_tokens = int(cu[-1]) if n_tokens is None else int(n_tokens)
             shape = (n_tokens, self.n_kv_heads, self.head_dim)
-            k = torch.empty(shape, dtype=torch.bfloat16, device=self.k.device)
+            k = torch.empty(*shape, dtype=torch.bfloat16, device=self.k.device)
             v = torch.empty_like(k)
         k, k_ptr, ldk, rows = self._rows(k, "k", copy=False)
         v, v_ptr, ldv, v_rows = self._rows(v, "v", copy=False)
