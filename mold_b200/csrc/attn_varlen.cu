@@ -1,14 +1,15 @@
 // K11: attention of packed prompts, causal or not, grouped heads, on tcgen05 + TMEM (sm_100a).
 //
-// One block = one 128-row query tile, two blocks on an SM: while one finds its work, waits for its first
+// Two blocks on an SM, each working on one 128-row query tile at a time: while one waits for its first
 // tiles or writes its output, the other computes (one block with two tiles, K4's layout, left the tensor
-// pipe at 32 % on a ragged batch).
+// pipe at 32 % on a ragged batch). A block takes over the work of blocks that have not started
+// (clusterlaunchcontrol), so that it finds the next tile and loads it under the present one.
 //   - A tile's rows are TQ = 128 / G tokens of all G query heads of one key head (row = token * G +
 //     head), one TMA box of G heads x TQ tokens: the group shares each K / V block, and a causal tile
 //     spans few tokens, so little of its diagonal blocks is masked work.
-//   - A block finds its sequence and tile from cu_q by a scan; a sequence's last tiles (the longest under
+//   - A tile's sequence and place are found from cu_q by a scan; a sequence's last tiles (the longest under
 //     a causal mask) come first.
-//   warp 0    TMA: the Q tile, then 64-key blocks of K and V into rings of their own.
+//   warp 0    next tile; TMA: the Q tile, then 64-key blocks of K and V into rings of their own.
 //   warp 1    MMA issuer. S(g) = Q K_g^T goes to one half of the S columns while the softmax works on the
 //             other: PV(g), then S(g + 2).
 //   warp 2    guards V: a P V product adds 0 * v for every masked key of a block, so in the blocks that a
@@ -19,6 +20,12 @@
 //             registers, P written back over S as bf16, lazy rescale of O. Only blocks that cross a row's
 //             limit are masked.
 // TMEM (256 columns a block): S [0, 128) in halves of 64, O [128, 128 + D).
+//
+// Bound by the softmax's chain on one thread a row (its exponentials alone take the tensor core's time)
+// and, in long runs, by the board's power. Measured and not kept: two softmax groups on alternate
+// blocks (568 against 542 us on one prompt of 8201 tokens, 32/8 heads: 16 softmax warps slow the issuer),
+// 128-key score products with two groups (607 us: one S buffer), K4's share of polynomial exponentials
+// (618 against 556 us), the output by TMA (no stage is free under the next tile's loads).
 #include <math.h>
 
 #include <string>
@@ -61,18 +68,23 @@ MB_DEV float max3_nan(float a, float b, float c) {
 }
 MB_DEV bool finite_bf16(uint32_t bits) { return (bits & 0x7f80u) != 0x7f80u; }
 
-// What a block works on. Computed by warp 0.
+// A tile, as warp 0 tells the others.
 struct Work {
+  int valid;             // 0: there is none left
+  int hk;                // key head
   int q_start, k_start;  // first packed row of the sequence
   int m, n;              // queries, keys
-  int tok0;              // first token of tile 0
+  int tok0;              // first token of the tile
 };
+constexpr int kWorkReaders = 6;  // MMA issuer, guard and four softmax warps
 
-// Sequence and tile of item `idx` (counting each sequence's tiles of `span` tokens); false behind the last.
-MB_DEV bool find_work(const Params& p, int64_t idx, int span, Work& w) {
+// Sequence and tile of item `idx` (counting each sequence's tiles of `span` tokens); false behind the last. With offsets
+// that overlap the sums may wrap; a tile outside its sequence is none.
+MB_DEV bool find_work(const Params& p, int idx, int span, Work& w) {
   const int lane = threadIdx.x & 31;
-  auto clampq = [&](int64_t x) { return (int)(x < 0 ? 0 : x < p.total_q ? x : p.total_q); };
-  auto clampk = [&](int64_t x) { return (int)(x < 0 ? 0 : x < p.total_k ? x : p.total_k); };
+  auto clampq = [&](int x) { return max(0, min(x, (int)p.total_q)); };
+  auto clampk = [&](int x) { return max(0, min(x, (int)p.total_k)); };
+#pragma unroll 1
   for (int base = 0; base < p.n_seqs; base += 32) {
     const int b = base + lane;
     int q0 = 0, m = 0, k0 = 0, n = 0;
@@ -82,26 +94,48 @@ MB_DEV bool find_work(const Params& p, int64_t idx, int span, Work& w) {
       k0 = clampk(__ldg(p.cu_k + b));
       n = max(0, clampk(__ldg(p.cu_k + b + 1)) - k0);
     }
-    int64_t x = (m + span - 1) / span;
+    int x = (m + span - 1) / span;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, idx < x);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int64_t end = __shfl_sync(0xffffffffu, x, src);
       w.q_start = __shfl_sync(0xffffffffu, q0, src);
       w.m = __shfl_sync(0xffffffffu, m, src);
       w.k_start = __shfl_sync(0xffffffffu, k0, src);
       w.n = __shfl_sync(0xffffffffu, n, src);
-      w.tok0 = (int)(end - 1 - idx) * span;  // last tile first
-      return true;
+      const int last = __shfl_sync(0xffffffffu, x, src) - 1 - idx;  // last tile first
+      w.tok0 = last * span;
+      return last >= 0 && last <= (w.m - 1) / span && w.m > 0;
     }
     idx -= __shfl_sync(0xffffffffu, x, 31);
   }
   return false;
+}
+
+// Asks for a block of this grid that has not started, to be cancelled: 16 bytes at `to`, counted by `bar`.
+MB_DEV void take_block(void* to, uint64_t* bar) {
+  fence_proxy_async_smem();  // the last answer has been read
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(to)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The cancelled block's index, whose work is the caller's now; -1: all have started.
+MB_DEV int taken_block(const void* from) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b128 r;\n .reg .b32 y, z, w;\n ld.shared.b128 r, [%2];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n}\n"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(from))
+      : "memory");
+  return ok ? (int)x : -1;
 }
 
 template <int D>
@@ -117,7 +151,7 @@ struct Smem {
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2)
     k_attention_varlen(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to, const Params p) {
+                       const __grid_constant__ CUtensorMap tv, const Params p) {
   using S = Smem<D>;
   constexpr int CH = D / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -126,52 +160,51 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* sV = sK + kK * S::kBlock;
   uint64_t* bars = (uint64_t*)(smem + S::kBars);
   uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;    // [kK]
-  uint64_t* k_empty = bars + 3;   // [kK]
-  uint64_t* v_full = bars + 5;    // [kV]
-  uint64_t* v_ok = bars + 8;      // [kV]: guarded blocks
-  uint64_t* v_empty = bars + 11;  // [kV]
-  uint64_t* s_full = bars + 14;   // [half]
-  uint64_t* p_full = bars + 16;   // [half]
-  uint64_t* o_full = bars + 18;
-  uint64_t* pv_done = bars + 19;  // one completion per P V product
-  uint32_t* tmem_slot = (uint32_t*)(bars + 20);
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;    // [kK]
+  uint64_t* k_empty = bars + 4;   // [kK]
+  uint64_t* v_full = bars + 6;    // [kV]
+  uint64_t* v_ok = bars + 9;      // [kV]: guarded
+  uint64_t* v_empty = bars + 12;  // [kV]
+  uint64_t* s_full = bars + 15;   // [half]
+  uint64_t* p_full = bars + 17;   // [half]
+  uint64_t* o_full = bars + 19;
+  uint64_t* pv_done = bars + 20;     // one completion per P V product
+  uint64_t* work_full = bars + 21;   // [2]
+  uint64_t* work_empty = bars + 23;  // [2]
+  uint64_t* next_bar = bars + 25;
+  uint8_t* next = (uint8_t*)(bars + 26);  // 16 bytes
+  Work* work = (Work*)(bars + 28);        // [2]
+  volatile int* odd_v = (volatile int*)(work + 2);  // [2]: a value that is not finite was zeroed for this tile
+  uint32_t* tmem_slot = (uint32_t*)(work + 2) + 2;
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  volatile int* odd_v = (volatile int*)(tmem_slot + 2);  // a value that is not finite was zeroed
-  int* found = (int*)(tmem_slot + 3);
-  Work* work = (Work*)(tmem_slot + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.G, TQ = p.TQ;
-  const int64_t item = blockIdx.x / p.Hkv;
-  const int hk = (int)(blockIdx.x - item * p.Hkv);
 
-  if (warp == 0) {
-    Work w;
-    const bool ok = find_work(p, item, TQ, w);
-    if (lane == 0) {
-      *found = ok;
-      if (ok) *work = w;
-      mbar_init(q_full, 1);
-      for (int i = 0; i < kK; i++) {
-        mbar_init(&k_full[i], 1);
-        mbar_init(&k_empty[i], 1);
-      }
-      for (int i = 0; i < kV; i++) {
-        mbar_init(&v_full[i], 1);
-        mbar_init(&v_ok[i], 1);
-        mbar_init(&v_empty[i], 2);  // the MMA issuer's and the guard's
-      }
-      for (int i = 0; i < 2; i++) {
-        mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 4);
-      }
-      mbar_init(o_full, 1);
-      mbar_init(pv_done, 1);
-      *abort_flag = 0;
-      *odd_v = 0;
-      fence_mbar_init();
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < kK; i++) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
     }
+    for (int i = 0; i < kV; i++) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_ok[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&work_full[i], 1);
+      mbar_init(&work_empty[i], kWorkReaders);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(pv_done, 1);
+    mbar_init(next_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
@@ -181,288 +214,346 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (!*found) {
-    if (warp == 1) tmem_dealloc(tmem, 256);
-    return;
-  }
-  const Work w = *work;
-
-  // keys that the mask leaves token i of the sequence: the first keys_of(i)
-  auto keys_of = [&](int i) { return p.causal ? max(0, min(i + 1 + w.n - w.m, w.n)) : w.n; };
-  const int all_see = keys_of(w.tok0);  // keys that every row sees
-  const int n_kv = (keys_of(min(w.tok0 + TQ, w.m) - 1) + BKV - 1) / BKV;
-  // blocks from this one on hold keys that some row is not to see
-  const int guard0 = all_see / BKV;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort_flag, p.status, kDevTimeoutAttn); };
+  // keys that the mask leaves token i of the sequence: the first keys_of(w, i)
+  auto keys_of = [&](const Work& w, int i) { return p.causal ? max(0, min(i + 1 + w.n - w.m, w.n)) : w.n; };
+  auto blocks_of = [&](const Work& w) { return (keys_of(w, min(w.tok0 + TQ, w.m) - 1) + BKV - 1) / BKV; };
+  // Every role walks the same tiles. Rings and phases run on over them: block g of a tile is block kb + g of all.
 
   if (warp == 0) {
-    if (lane == 0 && n_kv > 0) {
+    int block = blockIdx.x, qn = 0, kb = 0, asked = 0;
+    if (lane == 0) {
       tma_prefetch_desc(&tq);
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
-      mbar_expect_tx(q_full, (uint32_t)(CH * G * TQ * 128));
-      for (int c = 0; c < CH; c++)
-        tma_load_3d(sQ + c * S::kQHalf, &tq, q_full, c * 64, hk * G, w.q_start + w.tok0);
-      // V of block j - 1 after K of block j: the scores need their K first
-      int nk = 0, nv = 0;
-      for (int j = 0; j <= n_kv; j++) {
-        if (j < n_kv) {
-          const int s = j % kK;
-          if (!mbar_wait(&k_empty[s], ((j / kK) & 1) ^ 1, abort_flag, p.status, kDevTimeoutAttn)) break;
-          mbar_expect_tx(&k_full[s], S::kBlock);
-          for (int c = 0; c < CH; c++)
-            tma_load_3d(sK + s * S::kBlock + c * S::kHalf, &tk, &k_full[s], c * 64, hk, w.k_start + j * BKV);
-          nk++;
-        }
-        if (j > 0) {
-          const int i = j - 1, s = i % kV;
-          if (!mbar_wait(&v_empty[s], ((i / kV) & 1) ^ 1, abort_flag, p.status, kDevTimeoutAttn)) break;
-          mbar_expect_tx(&v_full[s], S::kBlock);
-          for (int c = 0; c < CH; c++)
-            tma_load_3d(sV + s * S::kBlock + c * S::kHalf, &tv, &v_full[s], c * 64, hk, w.k_start + i * BKV);
-          nv++;
+    }
+    bool ok = true;
+    int nk = 0, nv = 0;  // blocks loaded, of all tiles
+    for (int it = 0; ok; it++) {
+      Work w;
+      w.valid = 0;
+      if (block >= 0) {
+        const int item = block / p.Hkv;
+        w.valid = find_work(p, item, TQ, w);
+        w.hk = block - item * p.Hkv;
+      }
+      if (lane == 0) {
+        if ((ok = wait(&work_empty[it & 1], ((it >> 1) & 1) ^ 1))) {
+          work[it & 1] = w;
+          mbar_arrive(&work_full[it & 1]);
         }
       }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok || !w.valid) break;
+      const int n_kv = blocks_of(w);
+      if (lane == 0 && n_kv > 0) {
+        if ((ok = wait(q_empty, (qn & 1) ^ 1))) {
+          mbar_expect_tx(q_full, (uint32_t)(CH * G * TQ * 128));
+          for (int c = 0; c < CH; c++)
+            tma_load_3d(sQ + c * S::kQHalf, &tq, q_full, c * 64, w.hk * G, w.q_start + w.tok0);
+          qn++;
+        }
+        // V of block j - 1 after K of block j: the scores need their K first
+        for (int j = 0; j <= n_kv && ok; j++) {
+          if (j == n_kv - 1) {  // late, so that blocks with little left take what is left
+            take_block(next, next_bar);
+            asked++;
+          }
+          if (j < n_kv) {
+            const int s = (kb + j) % kK;
+            if (!(ok = wait(&k_empty[s], (((kb + j) / kK) & 1) ^ 1))) break;
+            mbar_expect_tx(&k_full[s], S::kBlock);
+            for (int c = 0; c < CH; c++)
+              tma_load_3d(sK + s * S::kBlock + c * S::kHalf, &tk, &k_full[s], c * 64, w.hk, w.k_start + j * BKV);
+            nk++;
+          }
+          if (j > 0) {
+            const int s = (kb + j - 1) % kV;
+            if (!(ok = wait(&v_empty[s], (((kb + j - 1) / kV) & 1) ^ 1))) break;
+            mbar_expect_tx(&v_full[s], S::kBlock);
+            for (int c = 0; c < CH; c++)
+              tma_load_3d(sV + s * S::kBlock + c * S::kHalf, &tv, &v_full[s], c * 64, w.hk, w.k_start + (j - 1) * BKV);
+            nv++;
+          }
+        }
+      }
+      kb += n_kv;
+      if (lane == 0 && ok) {
+        if (asked == it) {  // a tile without keys
+          take_block(next, next_bar);
+          asked++;
+        }
+        if ((ok = wait(next_bar, it & 1))) block = taken_block(next);
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      block = __shfl_sync(0xffffffffu, block, 0);
+    }
+    if (lane == 0) {
       // the block's memory must outlive its copies, whatever the other warps do
       volatile int never = 0;
-      mbar_wait(q_full, 0, &never, p.status, kDevTimeoutAttn);
-      for (int j = max(nk - kK, 0); j < nk; j++)
-        mbar_wait(&k_full[j % kK], (j / kK) & 1, &never, p.status, kDevTimeoutAttn);
-      for (int j = max(nv - kV, 0); j < nv; j++)
-        mbar_wait(&v_full[j % kV], (j / kV) & 1, &never, p.status, kDevTimeoutAttn);
+      auto drain = [&](uint64_t* bar, int n) {
+        if (n > 0) mbar_wait(bar, (n - 1) & 1, &never, p.status, kDevTimeoutAttn);
+      };
+      drain(next_bar, asked);
+      drain(q_full, qn);
+      for (int i = 0; i < kK; i++) drain(&k_full[i], (nk - i + kK - 1) / kK);
+      for (int i = 0; i < kV; i++) drain(&v_full[i], (nv - i + kV - 1) / kV);
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = idesc_bf16(128, BKV, false);
     constexpr uint32_t idesc_o = idesc_bf16(128, D, true);
     const uint32_t qa = smem_u32(sQ);
-    bool ok = n_kv > 0 && mbar_wait(q_full, 0, abort_flag, p.status, kDevTimeoutAttn);
-    // S(g) = Q K_g^T into S half g & 1
-    auto issue_s = [&](int g) {
-      const int s = g % kK;
-      if (!(ok = mbar_wait(&k_full[s], (g / kK) & 1, abort_flag, p.status, kDevTimeoutAttn))) return;
-      tc_fence_after();
-      const uint32_t ka = smem_u32(sK) + s * S::kBlock;
+    int kb = 0, qn = 0;
+    bool ok = true;
+    for (int it = 0; ok; it++) {
+      if (!(ok = wait(&work_full[it & 1], (it >> 1) & 1))) break;
+      const Work w = work[it & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&work_empty[it & 1]);
+      if (!w.valid) break;
+      const int n_kv = blocks_of(w);
+      if (n_kv == 0) continue;
+      // S(g) = Q K_g^T into S half (kb + g) & 1
+      auto issue_s = [&](int g) {
+        const int b = kb + g, s = b % kK;
+        if (!(ok = wait(&k_full[s], (b / kK) & 1))) return;
+        tc_fence_after();
+        const uint32_t ka = smem_u32(sK) + s * S::kBlock;
 #pragma unroll
-      for (int c = 0; c < CH; c++)
-        umma_ss_x4_elect(tmem + (g & 1) * 64, sw128_desc(qa + c * S::kQHalf, 16, 1024),
-                         sw128_desc(ka + c * S::kHalf, 16, 1024), idesc_s, c > 0);
-      if (lane == 0) {
-        umma_commit(&s_full[g & 1]);
-        umma_commit(&k_empty[s]);
+        for (int c = 0; c < CH; c++)
+          umma_ss_x4_elect(tmem + (b & 1) * 64, sw128_desc(qa + c * S::kQHalf, 16, 1024),
+                           sw128_desc(ka + c * S::kHalf, 16, 1024), idesc_s, c > 0);
+        if (lane == 0) {
+          umma_commit(&s_full[b & 1]);
+          umma_commit(&k_empty[s]);
+          if (g == n_kv - 1) umma_commit(q_empty);
+        }
+        __syncwarp();
+      };
+      if (!(ok = wait(q_full, qn & 1))) break;
+      issue_s(0);
+      if (ok && n_kv > 1) issue_s(1);
+      for (int g = 0; g < n_kv && ok; g++) {
+        const int b = kb + g, s = b % kV;
+        if (!(ok = wait(&p_full[b & 1], (b >> 1) & 1))) break;
+        if (!(ok = wait(&v_ok[s], (b / kV) & 1))) break;
+        tc_fence_after();
+        // O += P(g) V_g, P read from TMEM (bf16 pairs over the first 32 columns of its S half); V [keys, d] is MN-major:
+        // 64-wide d chunks kHalf apart, 8-key groups 1024 B apart. The first P of a tile comes after its softmax warps
+        // have read the last tile's O.
+        umma_ts_x4_elect(tmem + 128, tmem + (b & 1) * 64, sw128_desc(smem_u32(sV) + s * S::kBlock, S::kHalf, 1024), idesc_o,
+                         g > 0 ? 1u : 0u);
+        if (lane == 0) {
+          umma_commit(pv_done);
+          umma_commit(&v_empty[s]);
+          if (g == n_kv - 1) umma_commit(o_full);
+        }
+        __syncwarp();
+        if (g + 2 < n_kv) issue_s(g + 2);
       }
-      __syncwarp();
-    };
-    if (ok) issue_s(0);
-    if (ok && n_kv > 1) issue_s(1);
-    for (int g = 0; g < n_kv && ok; g++) {
-      const int s = g % kV;
-      if (!(ok = g < guard0
-                     ? mbar_wait(&v_full[s], (g / kV) & 1, abort_flag, p.status, kDevTimeoutAttn)
-                     : mbar_wait(&v_ok[s], ((g - guard0) / kV) & 1, abort_flag, p.status, kDevTimeoutAttn)))
-        break;
-      if (!(ok = mbar_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
-      tc_fence_after();
-      // O += P(g) V_g, P read from TMEM (bf16 pairs over the first 32 columns of its S half); V [keys, d] is MN-major:
-      // 64-wide d chunks kHalf apart, 8-key groups 1024 B apart
-      const uint32_t va = smem_u32(sV) + s * S::kBlock;
-      umma_ts_x4_elect(tmem + 128, tmem + (g & 1) * 64, sw128_desc(va, S::kHalf, 1024), idesc_o, g > 0 ? 1u : 0u);
-      if (lane == 0) {
-        umma_commit(pv_done);
-        umma_commit(&v_empty[s]);
-      }
-      __syncwarp();
-      if (g + 2 < n_kv) issue_s(g + 2);
+      kb += n_kv;
+      qn++;
     }
-    if (ok && lane == 0) umma_commit(o_full);
-    __syncwarp();
   } else if (warp == 2) {
     // ---------------------------------------------------------------- V guard
-    // Takes part in every block, so that it never falls a phase of a barrier behind.
-    for (int j = 0; j < n_kv; j++) {
-      const int s = j % kV;
-      if (!mbar_wait(&v_full[s], (j / kV) & 1, abort_flag, p.status, kDevTimeoutAttn)) break;
-      if (j >= guard0) {
-        uint8_t* v = sV + s * S::kBlock;
-        // 16-byte pieces by address: a row is 128 bytes of each atom column, and the swizzle moves pieces
-        // inside a row only
-        const int rows = min(BKV, w.n - j * BKV);
-        for (int i = rows * 8 + lane; i < BKV * 8; i += 32)
+    int kb = 0;
+    bool ok = true;
+    for (int it = 0; ok; it++) {
+      if (!(ok = wait(&work_full[it & 1], (it >> 1) & 1))) break;
+      const Work w = work[it & 1];
+      if (!w.valid) break;
+      if (lane == 0) odd_v[it & 1] = 0;
+      __syncwarp();
+      const int n_kv = blocks_of(w);
+      // blocks from this one on hold keys that some row is not to see
+      const int guard0 = keys_of(w, w.tok0) / BKV;
+      for (int j = 0; j < n_kv; j++) {
+        const int s = (kb + j) % kV;
+        if (!(ok = wait(&v_full[s], ((kb + j) / kV) & 1))) break;
+        if (j >= guard0) {
+          uint8_t* v = sV + s * S::kBlock;
+          // 16-byte pieces by address: a row is 128 bytes of each atom column, and the swizzle moves pieces
+          // inside a row only
+          const int rows = min(BKV, w.n - j * BKV);
+          for (int i = rows * 8 + lane; i < BKV * 8; i += 32)
 #pragma unroll
-          for (int c = 0; c < CH; c++) *(uint4*)(v + c * S::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
-        if (p.causal) {
-          __nv_bfloat162 acc = __float2bfloat162_rn(0.f);
-          const __nv_bfloat162 zero = acc;
-          for (int c = 0; c < CH; c++)
-#pragma unroll 4
-            for (int i = lane; i < rows * 8; i += 32) {
-              const uint4 x = *(const uint4*)(v + c * S::kHalf + i * 16);
-              acc = __hfma2(*(const __nv_bfloat162*)&x.x, zero, acc);  // NaN from what is not finite, and it stays
-              acc = __hfma2(*(const __nv_bfloat162*)&x.y, zero, acc);
-              acc = __hfma2(*(const __nv_bfloat162*)&x.z, zero, acc);
-              acc = __hfma2(*(const __nv_bfloat162*)&x.w, zero, acc);
-            }
-          const uint32_t bits = *(const uint32_t*)&acc;
-          if (!finite_bf16(bits) || !finite_bf16(bits >> 16)) {
-            *odd_v = 1;
+            for (int c = 0; c < CH; c++) *(uint4*)(v + c * S::kHalf + i * 16) = make_uint4(0, 0, 0, 0);
+          if (p.causal) {
+            __nv_bfloat162 acc = __float2bfloat162_rn(0.f);
+            const __nv_bfloat162 zero = acc;
             for (int c = 0; c < CH; c++)
+#pragma unroll 4
               for (int i = lane; i < rows * 8; i += 32) {
-                uint32_t* x = (uint32_t*)(v + c * S::kHalf + i * 16);
-                for (int e = 0; e < 4; e++) {
-                  uint32_t y = x[e];
-                  if (!finite_bf16(y)) y &= 0xffff0000u;
-                  if (!finite_bf16(y >> 16)) y &= 0x0000ffffu;
-                  x[e] = y;
-                }
+                const uint4 x = *(const uint4*)(v + c * S::kHalf + i * 16);
+                acc = __hfma2(*(const __nv_bfloat162*)&x.x, zero, acc);  // NaN from what is not finite, and it stays
+                acc = __hfma2(*(const __nv_bfloat162*)&x.y, zero, acc);
+                acc = __hfma2(*(const __nv_bfloat162*)&x.z, zero, acc);
+                acc = __hfma2(*(const __nv_bfloat162*)&x.w, zero, acc);
               }
+            const uint32_t bits = *(const uint32_t*)&acc;
+            if (!finite_bf16(bits) || !finite_bf16(bits >> 16)) {
+              odd_v[it & 1] = 1;
+              for (int c = 0; c < CH; c++)
+                for (int i = lane; i < rows * 8; i += 32) {
+                  uint32_t* x = (uint32_t*)(v + c * S::kHalf + i * 16);
+                  for (int e = 0; e < 4; e++) {
+                    uint32_t y = x[e];
+                    if (!finite_bf16(y)) y &= 0xffff0000u;
+                    if (!finite_bf16(y >> 16)) y &= 0x0000ffffu;
+                    x[e] = y;
+                  }
+                }
+            }
           }
+          fence_proxy_async_smem();
         }
-        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ok[s]);
       }
+      kb += n_kv;
       __syncwarp();
-      if (lane == 0) {
-        if (j >= guard0) mbar_arrive(&v_ok[s]);
-        mbar_arrive(&v_empty[s]);
-      }
-      __syncwarp();
+      if (lane == 0) mbar_arrive(&work_empty[it & 1]);
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- softmax
     const int r = (warp - 4) * 32 + lane;
     const uint32_t lane_addr = (uint32_t)((warp - 4) * 32) << 16;
     const uint32_t tO = tmem + 128 + lane_addr;
-    const int tok = w.tok0 + r / G, head = hk * G + r % G;
-    const bool mine = r < TQ * G && tok < w.m;  // this row is one of the sequence's
-    const int keys = keys_of(min(tok, w.m - 1));
+    const int row_tok = r / G, row_head = r % G;
     const float sc = p.scale_log2;
-    float m_run = -INFINITY, l_run = 0.f;
-    bool ok = true, ready = false;
-    for (int g = 0; g < n_kv; g++) {
-      if (!ready && !(ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
-      tc_fence_after();
-      const uint32_t tSh = tmem + (g & 1) * 64 + lane_addr;
-      uint32_t v[2][32];
-      tmem_ld32(tSh, v[0]);
-      tmem_ld32(tSh + 32, v[1]);
-      tmem_wait_ld();
-      const bool masked = (g + 1) * BKV > all_see;  // the same for the whole tile
-      if (masked) {
-        const int valid = keys - g * BKV;
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-          for (int i = 0; i < 32; i++)
-            if (c * 32 + i >= valid) v[c][i] = __float_as_uint(-INFINITY);
-      }
-      float mc[4];  // four independent chains
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        const uint32_t* x = &v[c >> 1][(c & 1) * 16];
-        mc[c] = max_nan(__uint_as_float(x[0]), __uint_as_float(x[1]));
-#pragma unroll
-        for (int i = 2; i < 16; i += 2) mc[c] = max3_nan(mc[c], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-      }
-      const float m_new = max_nan(m_run, max3_nan(mc[0], mc[1], max_nan(mc[2], mc[3])) * sc);
-      // lazy rescale: only rows whose max grew by more than 2^8 (or turned NaN) move their reference point
-      const bool need = g == 0 || !(m_new <= m_run + kRescaleThreshold);
-      const float alpha = (need && g > 0 && mine) ? ex2_approx(m_run - m_new) : 1.f;
-      if (need) m_run = m_new;
-      const float ref = m_run == -INFINITY ? 0.f : m_run;  // no key so far: weights 0
-      const uint64_t sc2 = pk2(sc, sc), nm2 = pk2(-ref, -ref);
-      uint64_t sum2 = pk2(0.f, 0.f);
-      // All exponentials on the MUFU pipe: with K4's share of 6 in 32 as polynomials on the FMA pipe this kernel lost 10 %
-      // (8201 tokens, 32/8 heads: 556 -> 618 us).
-#pragma unroll
-      for (int c = 0; c < 2; c++) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          const uint64_t x2 = fma2(pk2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sc2, nm2);
-          float x0, x1;
-          up2(x2, x0, x1);
-          const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
-          sum2 = add2(sum2, pk2(e0, e1));
-          pk[i] = pack_bf16x2(e0, e1);
-        }
-        tmem_st16a(tSh + c * 16, pk);
-      }
-      float sa, sb;
-      up2(sum2, sa, sb);
-      if (g > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        // O must hold P V of block g - 1 before it is rescaled
-        if (!(ok = mbar_wait(pv_done, (g - 1) & 1, abort_flag, p.status, kDevTimeoutAttn))) break;
+    int kb = 0, qn = 0;
+    bool ok = true;
+    for (int it = 0; ok; it++) {
+      if (!(ok = wait(&work_full[it & 1], (it >> 1) & 1))) break;
+      const Work w = work[it & 1];
+      if (!w.valid) break;
+      const int n_kv = blocks_of(w);
+      const int all_see = keys_of(w, w.tok0);  // keys that every row sees
+      const int tok = w.tok0 + row_tok;
+      const bool mine = r < TQ * G && tok < w.m;  // this row is one of the sequence's
+      const int keys = keys_of(w, min(tok, w.m - 1));
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int g = 0; g < n_kv; g++) {
+        const int b = kb + g;
+        if (!(ok = wait(&s_full[b & 1], (b >> 1) & 1))) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < D / 32; c++) {
-          uint32_t o[32];
-          tmem_ld32(tO + c * 32, o);
-          tmem_wait_ld();
+        const uint32_t tSh = tmem + (b & 1) * 64 + lane_addr;
+        uint32_t v[2][32];
+        tmem_ld32(tSh, v[0]);
+        tmem_ld32(tSh + 32, v[1]);
+        tmem_wait_ld();
+        const bool masked = (g + 1) * BKV > all_see;  // the same for the whole tile
+        if (masked) {
 #pragma unroll
-          for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(tO + c * 32, o);
+          for (int c = 0; c < 2; c++) {
+            const int valid = keys - g * BKV - c * 32;
+            const uint32_t bits = valid <= 0 ? 0u : valid >= 32 ? 0xffffffffu : (1u << valid) - 1u;
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              if (!((bits >> i) & 1)) v[c][i] = __float_as_uint(-INFINITY);
+          }
         }
+        float mc[4];  // four independent chains
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const uint32_t* x = &v[c >> 1][(c & 1) * 16];
+          mc[c] = max_nan(__uint_as_float(x[0]), __uint_as_float(x[1]));
+#pragma unroll
+          for (int i = 2; i < 16; i += 2) mc[c] = max3_nan(mc[c], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        }
+        const float m_new = max_nan(m_run, max3_nan(mc[0], mc[1], max_nan(mc[2], mc[3])) * sc);
+        // lazy rescale: only rows whose max grew by more than 2^8 (or turned NaN) move their reference point
+        const bool need = g == 0 || !(m_new <= m_run + kRescaleThreshold);
+        const float alpha = (need && g > 0 && mine) ? ex2_approx(m_run - m_new) : 1.f;
+        if (need) m_run = m_new;
+        const float ref = m_run == -INFINITY ? 0.f : m_run;  // no key so far: weights 0
+        const uint64_t sc2 = pk2(sc, sc), nm2 = pk2(-ref, -ref);
+        uint64_t sum2 = pk2(0.f, 0.f);
+        // All exponentials on the MUFU pipe: with K4's share of 6 in 32 as polynomials on the FMA pipe this kernel lost 10 %
+        // (8201 tokens, 32/8 heads: 556 -> 618 us).
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const uint64_t x2 = fma2(pk2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), sc2, nm2);
+            float x0, x1;
+            up2(x2, x0, x1);
+            const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
+            sum2 = add2(sum2, pk2(e0, e1));
+            pk[i] = pack_bf16x2(e0, e1);
+          }
+          tmem_st16a(tSh + c * 16, pk);
+        }
+        float sa, sb;
+        up2(sum2, sa, sb);
+        if (g > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // O must hold P V of block g - 1 before it is rescaled
+          if (!(ok = wait(pv_done, (b - 1) & 1))) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; c++) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(tO + c * 32, o);
+          }
+        }
+        tmem_wait_st();
+        l_run = l_run * alpha + (sa + sb);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[b & 1]);
       }
-      // the next scores are usually there: ask while the stores are on their way
-      ready = g + 1 < n_kv && mbar_try_wait(&s_full[(g + 1) & 1], ((g + 1) >> 1) & 1);
-      tmem_wait_st();
-      l_run = l_run * alpha + (sa + sb);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[g & 1]);
-    }
-    if (ok && n_kv > 0) ok = mbar_wait(o_full, 0, abort_flag, p.status, kDevTimeoutAttn);
-    // A tile whose tokens all belong to the sequence is gathered in the Q tile's place (its last product is done) and
-    // stored by TMA, row by row by its threads otherwise (4400 cycles for every tile when all were).
-    const bool whole = w.tok0 + TQ <= w.m;
-    if (ok) {
+      if (ok && n_kv > 0) ok = wait(o_full, qn & 1);
+      if (!ok) break;
+      kb += n_kv;
+      qn += n_kv > 0;
       tc_fence_after();
       // a row without keys is 0; a maximum of NaN or +inf, or -inf over keys, makes softmax NaN
       const float inv = keys <= 0 ? 0.f : fabsf(m_run) < INFINITY ? 1.f / l_run : __uint_as_float(0x7fc00000u);
-      __nv_bfloat16* orow = p.out + (int64_t)(w.q_start + tok) * p.ldo + (int64_t)head * D;
-      const bool odd = *odd_v;
+      __nv_bfloat16* orow = p.out + (int64_t)(w.q_start + tok) * p.ldo + (int64_t)(w.hk * G + row_head) * D;
 #pragma unroll 1
       for (int c = 0; c < D / 32; c++) {
         uint32_t o[32];
         if (n_kv > 0) {
           tmem_ld32(tO + c * 32, o);
           tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[i] = 0u;
         }
+        if (mine) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) o[i] = keys > 0 ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
-        if (odd) {
-#pragma unroll 1
-          for (int key = guard0 * BKV; key < keys; key++) {
-            const uint32_t* src =
-                (const uint32_t*)(p.v + (int64_t)(w.k_start + key) * p.ldv + (int64_t)hk * D + c * 32);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const uint32_t y = __ldg(src + i);
-              if (!finite_bf16(y)) o[2 * i] = __float_as_uint(__uint_as_float(o[2 * i]) + bf16_lo(y));
-              if (!finite_bf16(y >> 16)) o[2 * i + 1] = __float_as_uint(__uint_as_float(o[2 * i + 1]) + bf16_hi(y));
-            }
+          for (int u = 0; u < 4; u++) {
+            uint4 w4;
+            w4.x = pack_bf16x2(__uint_as_float(o[8 * u + 0]), __uint_as_float(o[8 * u + 1]));
+            w4.y = pack_bf16x2(__uint_as_float(o[8 * u + 2]), __uint_as_float(o[8 * u + 3]));
+            w4.z = pack_bf16x2(__uint_as_float(o[8 * u + 4]), __uint_as_float(o[8 * u + 5]));
+            w4.w = pack_bf16x2(__uint_as_float(o[8 * u + 6]), __uint_as_float(o[8 * u + 7]));
+            *(uint4*)(orow + c * 32 + u * 8) = w4;
           }
         }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          uint4 w4;
-          w4.x = pack_bf16x2(__uint_as_float(o[8 * u + 0]), __uint_as_float(o[8 * u + 1]));
-          w4.y = pack_bf16x2(__uint_as_float(o[8 * u + 2]), __uint_as_float(o[8 * u + 3]));
-          w4.z = pack_bf16x2(__uint_as_float(o[8 * u + 4]), __uint_as_float(o[8 * u + 5]));
-          w4.w = pack_bf16x2(__uint_as_float(o[8 * u + 6]), __uint_as_float(o[8 * u + 7]));
-          if (whole)
-            *(uint4*)(sQ + (c >> 1) * S::kQHalf + r * 128 + ((((c & 1) * 4 + u) ^ (r & 7)) << 4)) = w4;
-          else if (mine)
-            *(uint4*)(orow + c * 32 + u * 8) = w4;
+      }
+      if (odd_v[it & 1] && mine) {
+        // values that are not finite and that the row sees; one by one, since this hardly ever runs
+#pragma unroll 1
+        for (int key = all_see / BKV * BKV; key < keys; key++) {
+          const __nv_bfloat16* src = p.v + (int64_t)(w.k_start + key) * p.ldv + (int64_t)w.hk * D;
+#pragma unroll 1
+          for (int i = 0; i < D; i++) {
+            const float y = __bfloat162float(src[i]);
+            if (!(fabsf(y) < INFINITY)) orow[i] = __float2bfloat16_rn(__bfloat162float(orow[i]) + y);
+          }
         }
       }
-    }
-    if (whole) {
-      fence_proxy_async_smem();
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // the softmax warps, which all come here
-      if (warp == 4 && lane == 0 && ok) {
-        for (int c = 0; c < CH; c++)
-          tma_store_3d(&to, sQ + c * S::kQHalf, c * 64, hk * G, w.q_start + w.tok0);
-        bulk_commit();
-        bulk_wait_read();
-      }
+      tc_fence_before();  // O has been read: the next tile's first P, and the product after it, follow
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&work_empty[it & 1]);
     }
   }
 
@@ -476,13 +567,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 template <int D>
 cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, int64_t ldk, int H, cudaStream_t st) {
-  CUtensorMap tq, tk, tv, to;
+  CUtensorMap tq, tk, tv;
   const uint64_t head = D * 2, keys = p.total_k > 0 ? (uint64_t)p.total_k : 1;
   // {channel, head, token}; a sequence's end inside a box reads the next sequence's rows, which the masks leave out
   if (!make_tmap_3d(&tq, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)H, (uint64_t)p.total_q, head,
                     (uint64_t)ldq * 2, 64, (uint32_t)p.G, (uint32_t)p.TQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_3d(&to, p.out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)H, (uint64_t)p.total_q, head,
-                    (uint64_t)p.ldo * 2, 64, (uint32_t)p.G, (uint32_t)p.TQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tmap_3d(&tk, k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)p.Hkv, keys, head,
                     (uint64_t)ldk * 2, 64, 1, BKV, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tmap_3d(&tv, p.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)p.Hkv, keys, head,
@@ -499,7 +588,7 @@ cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, i
   }
   const int64_t blocks = (p.total_q / p.TQ + p.n_seqs) * p.Hkv;  // each sequence rounds up once
   if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  k_attention_varlen<D><<<(unsigned)blocks, kThreads, Smem<D>::kBytes, st>>>(tq, tk, tv, to, p);
+  k_attention_varlen<D><<<(unsigned)blocks, kThreads, Smem<D>::kBytes, st>>>(tq, tk, tv, p);
   return cudaGetLastError();
 }
 
