@@ -2,8 +2,9 @@
 // with a scale a row), split over the cached length and joined.
 //
 // Work is counted in tiles of kTileKeys keys of one unit = (sequence, key head, up to 16 of the query
-// heads that read it). The tiles of all units in a row are cut into equal runs, one for each block of a
-// grid that fills the SMs, so blocks end together however far the lengths lie apart. A block's part of a
+// heads that read it), and kUnitCost for a unit's own expense. All units in a row are cut into runs of
+// equal cost, one for each block of a grid that fills the SMs, so blocks end together however far the
+// lengths lie apart. A block's part of a
 // unit that it does not hold whole goes to the workspace as (max, sum, unnormalised output); k_join adds
 // a unit's parts in the order of the blocks.
 //
@@ -45,8 +46,14 @@ constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kRows = 16;                   // query rows of a unit
 constexpr int kMaxBlocksPerSm = 3;
 constexpr int kTileKeys = 16 * kWarps;
+constexpr int kCluster = 8;
 constexpr float kSlack = 4.f;               // log2 of how far a weight may pass 1
 constexpr float kWeightOne = 2048.f;        // f16 form of a weight of 1 with the largest value scale: 2^15 at most
+
+// Cost of a tile. A unit costs Shape::UNIT_COST besides its tiles (queries, joining the warps, output), more beside the
+// smaller tiles of an 8-bit cache. Without it blocks with many short units end last: 64 sequences up to 4096, bf16, cost
+// 0 / 3 / 6 / 12: 55.4 / 51.3 / 51.6 / 52.8 us; 160 up to 8192, e4m3, 0 / 3 / 8 / 12: 177 / 169 / 162 / 163 us.
+constexpr int kTileCost = 4;
 
 struct Part {  // of a unit's work: its first block and how many blocks hold a piece (1: none is joined)
   int first, pieces;
@@ -86,6 +93,12 @@ MB_DEV void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A float of another block of the cluster, at the place of p in this one.
+MB_DEV float ld_cluster(const float* p, int rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(smem_in_cta(p, rank)) : "memory");
+  return x;
 }
 // 32 channels of int8 codes; exact.
 MB_DEV void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -159,6 +172,7 @@ struct Shape {
   static constexpr int NR = WIDE ? 2 : 4;           // 16-channel output tiles that are merged at a time
   static constexpr int MERGE_PITCH = NR * 16 + 4;   // floats; rows 2t begin 8 banks apart
   static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
+  static constexpr int UNIT_COST = CODES == MB_KV_BF16 ? 3 : 8;
   static constexpr int BLOCKS = CODES == MB_KV_BF16 || WIDE ? 2 : 3;  // on an SM
   static constexpr int kBudget = (228 / BLOCKS - 2) * 1024;  // of a block: 1 KB is the system's, 1 KB for alignment
   static constexpr int kFixed = QSLOTS * QB + MERGEB + 2 * kWarps * kRows * 4 + 1024;  // and barriers, descriptors
@@ -166,6 +180,12 @@ struct Shape {
   static constexpr size_t kSmem = 1024 + (size_t)STAGES * STAGEB + kFixed;
   static_assert(STAGES >= 2, "ring too short");
 
+  // cost of a unit of nt tiles; tiles of the unit at `at` that begin before x
+  static MB_DEV int64_t unit_cost(int64_t nt) { return nt > 0 ? UNIT_COST + kTileCost * nt : 0; }
+  static MB_DEV int tiles_before(int64_t at, int64_t nt, int64_t x) {
+    const int64_t n = (x - at - UNIT_COST + kTileCost - 1) / kTileCost;
+    return x <= at + UNIT_COST ? 0 : (int)(n < nt ? n : nt);
+  }
   static MB_DEV uint32_t at(int key, int byte) {  // of a row's byte in K or V, swizzled
     const uint32_t off = (uint32_t)(key * LINEB + (byte & 127));
     return (uint32_t)(byte >> 7) * PLANEB + (off ^ ((off >> 3) & 0x70));
@@ -189,15 +209,15 @@ struct Desc {
   int last;         // the unit's last tile in this run
   int seq, unit;
   int slot;         // last: workspace slot for the part; -1: the unit is whole
-  int pad;
+  int end;          // the block's last tile
 };
 
-// Run of tiles of block c of n
+// Where block c of n begins in the row of units; a tile is done by the block in whose run its cost begins.
 MB_DEV int64_t run_start(int64_t total, int c, int n) { return total * c / n; }
-// The block whose run holds tile t
-MB_DEV int run_owner(int64_t total, int64_t t, int n) { return (int)(((t + 1) * n - 1) / total); }
+MB_DEV int run_owner(int64_t total, int64_t at, int n) { return (int)(((at + 1) * n - 1) / total); }
 
-template <int CODES, int D, bool WIDE>
+// CLUSTER: kCluster blocks share one unit, evenly, and join in their shared memory; no workspace, no second launch.
+template <int CODES, int D, bool WIDE, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     k_attention_paged(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const Params p) {
   using S = Shape<CODES, D, WIDE>;
@@ -205,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
   constexpr int RR = WIDE ? 2 : 1;  // eights of query rows
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  float* part = (float*)smem;  // CLUSTER, once all tiles are done: [ROWS][D] outputs, [ROWS] maxima, [ROWS] sums
   uint8_t* s_q = smem + (size_t)STAGES * S::STAGEB;
   float* s_merge = (float*)(s_q + S::QSLOTS * S::QB);
   float* s_m = s_merge + S::MERGEB / 4;  // [kWarps][kRows]
@@ -239,50 +260,73 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     return n < 0 ? 0 : n < cap ? n : cap;
   };
   auto tiles_of = [&](int64_t len) { return (len + kTileKeys - 1) / kTileKeys; };
-  // tiles of sequences base .. base + threadIdx.x together (block-wide), and of all kThreads
-  auto scan = [&](int base, int64_t& all) {
-    int64_t x = tiles_of(length(base + (int)threadIdx.x)) * U;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) s_sum[warp] = x;
-    __syncthreads();
-    all = 0;
-#pragma unroll
-    for (int w = 0; w <= kWarps; w++) {
-      if (w < warp) x += s_sum[w];
-      all += s_sum[w];
-    }
-    return x;
-  };
-
-  int64_t total = 0, all, incl = 0;
-  for (int base = 0; base < p.n_seqs; base += kThreads) {
-    incl = scan(base, all);
-    total += all;
-  }
+  // The run: from position x0 to x1 of a row of units of cost `total`, first unit (b, unit) at `at`.
   const int c = blockIdx.x;
-  // sequences without positions: their rows are 0
-  for (int b = c; b < p.n_seqs; b += gridDim.x)
-    if (length(b) == 0)
-      for (int i = threadIdx.x; i < p.H * D / 8; i += kThreads) *((uint4*)(p.out + b * p.ldo) + i) = make_uint4(0, 0, 0, 0);
-  // every block of a run has a tile, so that the blocks between a unit's first and last hold pieces of it
-  const int n_blocks = (int)(total < gridDim.x ? total : gridDim.x);
-  if (c >= n_blocks) return;
-  const int64_t t0 = run_start(total, c, n_blocks), t1 = run_start(total, c + 1, n_blocks);
-  int64_t before = 0;
-  for (int base = 0;; base += kThreads) {
-    if (p.n_seqs > kThreads) incl = scan(base, all); else all = total;
-    const int64_t own = tiles_of(length(base + (int)threadIdx.x)) * U;
-    const int64_t end = before + incl;
-    if (t0 < end && t0 >= end - own) *s_seq = base + threadIdx.x, *s_at = end - own;
-    before += all;
-    if (t0 < before) break;
+  int b, unit, n_blocks = 1;
+  int64_t len, nt, at = 0, x0, x1, total = 0;
+  const int rank = CLUSTER ? (int)cluster_rank() : 0;
+  if constexpr (CLUSTER) {
+    const int u = c / kCluster;
+    b = u / U, unit = u - b * U;
+    len = length(b), nt = tiles_of(len);
+    total = S::unit_cost(nt);
+    const int64_t first = nt * rank / kCluster, end = nt * (rank + 1) / kCluster;
+    x0 = S::UNIT_COST + kTileCost * first, x1 = first < end ? S::UNIT_COST + kTileCost * end : x0;
+    __syncthreads();  // the barriers are initialised
+  } else {
+    // cost of sequences base .. base + threadIdx.x together (block-wide), and of all kThreads
+    auto scan = [&](int base, int64_t& all) {
+      int64_t x = S::unit_cost(tiles_of(length(base + (int)threadIdx.x))) * U;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) s_sum[warp] = x;
+      __syncthreads();
+      all = 0;
+#pragma unroll
+      for (int w = 0; w <= kWarps; w++) {
+        if (w < warp) x += s_sum[w];
+        all += s_sum[w];
+      }
+      return x;
+    };
+
+    int64_t all, incl = 0;
+    for (int base = 0; base < p.n_seqs; base += kThreads) {
+      incl = scan(base, all);
+      total += all;
+    }
+    // sequences without positions: their rows are 0
+    for (int b = c; b < p.n_seqs; b += gridDim.x)
+      if (length(b) == 0)
+        for (int i = threadIdx.x; i < p.H * D / 8; i += kThreads) *((uint4*)(p.out + b * p.ldo) + i) = make_uint4(0, 0, 0, 0);
+    // A run is a tile's cost at least, so that every block between a unit's first and last holds a piece of it.
+    n_blocks = (int)(total / kTileCost < gridDim.x ? total / kTileCost : gridDim.x);
+    if (c >= n_blocks) return;
+    x0 = run_start(total, c, n_blocks), x1 = run_start(total, c + 1, n_blocks);
+    int64_t before = 0;
+    for (int base = 0;; base += kThreads) {
+      if (p.n_seqs > kThreads) incl = scan(base, all); else all = total;
+      const int64_t own = S::unit_cost(tiles_of(length(base + (int)threadIdx.x))) * U;
+      const int64_t end = before + incl;
+      if (x0 < end && x0 >= end - own) *s_seq = base + threadIdx.x, *s_at = end - own;
+      before += all;
+      if (x0 < before) break;
+    }
+    __syncthreads();
+    // the first unit of the run, and whether any tile begins in it
+    b = *s_seq;
+    len = length(b), nt = tiles_of(len), at = *s_at;
+    if (nt == 0) return;  // lengths that changed under the call
+    unit = (int)((x0 - at) / S::unit_cost(nt));
+    at += unit * S::unit_cost(nt);
+    if (S::tiles_before(at, nt, x0) >= S::tiles_before(at, nt, x1) &&
+        (at + S::unit_cost(nt) >= total || at + S::unit_cost(nt) + S::UNIT_COST >= x1))
+      return;
   }
-  __syncthreads();
 
   if (warp == kWarps) {
     // ---------------------------------------------------------------- loads
@@ -290,30 +334,20 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
     }
-    int b = *s_seq, n_seg = 0, it = 0;
-    int64_t at = *s_at, tile = t0;
+    int n_seg = 0, it = 0;
     bool ok = true;
-    while (tile < t1 && ok) {
-      int64_t len = length(b);
-      int64_t nt = tiles_of(len);
-      while (tile >= at + nt * U && b < p.n_seqs) {  // next sequence that has tiles
-        at += nt * U;
-        len = length(++b);
-        nt = tiles_of(len);
-      }
-      if (b >= p.n_seqs) break;  // lengths that changed under the call
-      const int unit = (int)((tile - at) / nt);
-      const int64_t unit_at = at + unit * nt;
-      const int64_t last = min(t1, unit_at + nt);
-      const int kt0 = (int)(tile - unit_at), kt1 = (int)(last - unit_at);
+    while (ok && at + S::UNIT_COST < x1) {
+      const int kt0 = S::tiles_before(at, nt, x0), kt1 = S::tiles_before(at, nt, x1);
+      const int64_t next_at = at + S::unit_cost(nt);
+      const bool end = next_at >= total || next_at + S::UNIT_COST >= x1;
       const int hk = unit / p.q_tiles, qt = unit - hk * p.q_tiles;
       const int rows = min(kRows, p.G - qt * kRows);
       const bool whole = kt0 == 0 && kt1 == nt;
       const int32_t* table = p.table + (int64_t)b * p.ld_table;
-      if (kt0 == 0 && lane == 0) {
+      if (!CLUSTER && kt0 == 0 && kt1 > 0 && lane == 0) {
         Part part;
         part.first = c;
-        part.pieces = whole ? 1 : run_owner(total, unit_at + nt - 1, n_blocks) - c + 1;
+        part.pieces = whole ? 1 : run_owner(total, at + S::UNIT_COST + kTileCost * (nt - 1), n_blocks) - c + 1;
         p.parts[(int64_t)b * U + unit] = part;
       }
       const int qs = n_seg % S::QSLOTS;
@@ -343,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
           d.seq = b;
           d.unit = unit;
           d.slot = whole ? -1 : 2 * c + (kt0 == 0 ? 1 : 0);
-          d.pad = 0;
+          d.end = d.last && end;
           desc[s] = d;
           mbar_expect_tx(&full[s], __popc(groups) * 2u * (16 * S::ROWB + S::SCALEB / kWarps) + q_bytes);
         }
@@ -366,317 +400,355 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
         if (lane == 31 && q_bytes)
           bulk_load(s_q + qs * S::QB, p.q + (int64_t)b * p.ldq + (int64_t)(hk * p.G + qt * kRows) * D, q_bytes, &full[s]);
       }
-      n_seg++;
-      tile = last;
+      n_seg += kt0 < kt1;
+      at = next_at;
+      if (++unit == U) {  // next sequence that has tiles
+        unit = 0;
+        do {
+          len = length(++b);
+          nt = tiles_of(len);
+        } while (nt == 0 && b < p.n_seqs);
+        if (b >= p.n_seqs) break;
+      }
     }
     // the block's memory must outlive its copies, whatever the other warps do
     volatile int never = 0;
     for (int i = it < STAGES ? 0 : it - STAGES; i < it; i++)
       mbar_wait(&full[i % STAGES], (i / STAGES) & 1, &never, p.status, kDevTimeoutAttn);
-    return;
-  }
-
-  // ---------------------------------------------------------------- products
-  // Query operand of row 8 r + g, by four-channel groups: two pairs (bf16; f16 for e4m3), or a high and a low digit word
-  // (int8); and what brings the scores of rows 8 r + 2t and + 1 back to size, times log2(e).
-  constexpr bool B16 = CODES == MB_KV_BF16, I8 = CODES == MB_KV_I8;
-  uint32_t qa[RR][QW][2];
-  float q_size[RR][2];
-  // o: channels 16 i + g (0, 1) and + 8 (2, 3) of rows 8 r + 2t and + 1; m, l: of these rows
-  float o[RR][D / 16][4], m[RR][2], l[RR][2];
-  float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and kWeightOne over it
-  uint32_t merges = 0;
-  const int n_it = (int)(t1 - t0);
-  for (int it = 0; it < n_it; it++) {
-    const int s = it % STAGES;
-    if (!mbar_wait(&full[s], (it / STAGES) & 1, abort_flag, p.status, kDevTimeoutAttn)) break;
-    const Desc d = desc[s];
-    uint8_t* sk = smem + (size_t)s * S::STAGEB;
-    uint8_t* sv = sk + S::KVB;
-    if (d.q_slot >= 0) {
-      const int rows = min(kRows, p.G - (d.unit % p.q_tiles) * kRows);
-#pragma unroll
-      for (int r = 0; r < RR; r++) {
-        const bool have = g + 8 * r < rows;
-        const uint8_t* src = s_q + d.q_slot * S::QB + (g + 8 * r) * D * 2;
-        uint32_t top = 0;  // largest magnitude's bits: non-negative floats order like integers, NaN last
-#pragma unroll
-        for (int i = 0; i < QW; i++) {
-          uint2 x = make_uint2(0, 0);
-          if (have) x = *(const uint2*)(src + S::q_channel(i, t) * 2);
-          qa[r][i][0] = x.x, qa[r][i][1] = x.y;
-          if (!B16) {
-            top = max(top, max((x.x << 16) & 0x7fff0000u, (x.y << 16) & 0x7fff0000u));
-            top = max(top, max(x.x & 0x7fff0000u, x.y & 0x7fff0000u));
-          }
-        }
-        float back = 1.f;
-        if (!B16) {
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          float f;
-          if (I8) {
-            // below 2^-100 the row counts as 0
-            const bool some = top >= 0x0d800000u;
-            f = some ? 32639.f / __uint_as_float(top) : 0.f;
-            back = some ? __uint_as_float(top) / 32639.f : 0.f;
-          } else {  // to [1, 2) by a power of two
-            const int e = min(max((int)(top >> 23), 1), 253);
-            f = __uint_as_float((uint32_t)(254 - e) << 23);
-            back = __uint_as_float((uint32_t)e << 23);
-          }
-          if (top >= 0x7f800000u) f = 0.f, back = __uint_as_float(0x7fc00000u);  // NaN or infinity in the row
-#pragma unroll
-          for (int i = 0; i < QW; i++) {
-            if (I8) {
-              uint32_t h, w;
-              query_digits(make_uint2(qa[r][i][0], qa[r][i][1]), f, h, w);
-              qa[r][i][0] = h, qa[r][i][1] = w;
-            } else {
-              qa[r][i][0] = scaled_f16x2(qa[r][i][0], f), qa[r][i][1] = scaled_f16x2(qa[r][i][1], f);
-            }
-          }
-        }
-        back *= p.scale_log2;
-        q_size[r][0] = __shfl_sync(0xffffffffu, back, 8 * t), q_size[r][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.f;
-        m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.f;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[d.q_slot]);
-      v_ref = v_inv = 0.f;
-    }
-    const int key0 = warp * 16;
-    if ((d.groups >> warp) & 1) {
-      const int left = d.left - key0;  // of this warp's 16 keys; > 0
-      // 8-bit values are read ahead of the scores, whose latency hides theirs; where 16 rows leave no registers for
-      // them, when their turn comes
-      uint32_t vw[B16 ? 1 : D / 32][4];
-      auto load_v = [&](int i) {
-        ldmatrix_b8_x2_trans(smem_u32(sv + S::at(key0 + (lane & 15), (2 * i + (lane >> 4)) * 16)), vw[B16 ? 0 : i]);
-      };
-      if (!B16 && !WIDE) {
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) load_v(i);
-      }
-      // scores: sc[r][2 u + e] of key key_of(u, g) and row 8 r + 2t + e
-      const int key_a = S::key_of(0, g), key_b = S::key_of(1, g);
-      float sc[RR][4];
-      int hi[RR][4], lo[RR][4];
-#pragma unroll
-      for (int r = 0; r < RR; r++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) sc[r][e] = 0.f, hi[r][e] = lo[r][e] = 0;
-      constexpr int LB = S::LINEB / 4;  // a lane's bytes of a row in a line
-#pragma unroll
-      for (int pl = 0; pl < S::PLANES; pl++) {
-        uint32_t wa[LB / 4], wb[LB / 4];
-#pragma unroll
-        for (int i = 0; i < LB / 16; i++) {
-          const uint4 x = *(const uint4*)(sk + S::at(key0 + key_a, pl * 128 + t * LB + i * 16));
-          const uint4 y = *(const uint4*)(sk + S::at(key0 + key_b, pl * 128 + t * LB + i * 16));
-          wa[4 * i] = x.x, wa[4 * i + 1] = x.y, wa[4 * i + 2] = x.z, wa[4 * i + 3] = x.w;
-          wb[4 * i] = y.x, wb[4 * i + 1] = y.y, wb[4 * i + 2] = y.z, wb[4 * i + 3] = y.w;
-        }
-        if (CODES == MB_KV_E4M3) {
-#pragma unroll
-          for (int i = 0; i < LB / 4; i++) {
-            uint32_t a[4];
-            codes_f16<CODES>(wa[i], a[0], a[2]);
-            codes_f16<CODES>(wb[i], a[1], a[3]);
-#pragma unroll
-            for (int r = 0; r < RR; r++) mma16816_f16(sc[r], a[0], a[1], a[2], a[3], qa[r][i][0], qa[r][i][1]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < LB / 8; i++)
-#pragma unroll
-            for (int r = 0; r < RR; r++) {
-              if (B16) {
-                const uint32_t* q = qa[r][B16 ? pl * 4 + i : 0];
-                mma16816(sc[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], q[0], q[1]);
-              } else {
-                const int x = B16 ? 0 : 2 * i, y = B16 ? 0 : 2 * i + 1;
-                mma16832(hi[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], qa[r][x][0], qa[r][y][0]);
-                mma16832(lo[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], qa[r][x][1], qa[r][y][1]);
-              }
-            }
-        }
-      }
-      // scales of the two keys; those of rows that do not exist may be anything
-      const bool in_a = key_a < left, in_b = key_b < left;
-      float ks_a = 1.f, ks_b = 1.f, vs_a = 1.f, vs_b = 1.f;
-      if (!B16) {
-        const float* scale = (const float*)(sk + 2 * S::KVB) + key0;
-        ks_a = scale[key_a], ks_b = scale[key_b];
-        vs_a = in_a ? scale[kTileKeys + key_a] : 0.f, vs_b = in_b ? scale[kTileKeys + key_b] : 0.f;
-      }
-      // The reference points move (and the output with them) only when a score passes its row's by more than 2^kSlack,
-      // or a value scale the largest so far.
-      bool move = !B16 && fmaxf(vs_a, vs_b) > v_ref;
-#pragma unroll
-      for (int r = 0; r < RR; r++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          if (I8) {  // below 2^30
-            sc[r][e] = (float)(hi[r][e] * 256 + lo[r][e]);
-            sc[r][2 + e] = (float)(hi[r][2 + e] * 256 + lo[r][2 + e]);
-          }
-          sc[r][e] = in_a ? sc[r][e] * (ks_a * q_size[r][e]) : -INFINITY;
-          sc[r][2 + e] = in_b ? sc[r][2 + e] * (ks_b * q_size[r][e]) : -INFINITY;
-          move |= fmaxf(sc[r][e], sc[r][2 + e]) > m[r][e] + kSlack;
-        }
-      if (__any_sync(0xffffffffu, move)) {
-        float shrink = 1.f;
-        if (!B16) {
-          float vm = fmaxf(vs_a, vs_b);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, x));
-          if (vm > v_ref) {  // the same in all lanes
-            shrink = v_ref / vm;
-            v_ref = vm;
-            v_inv = kWeightOne / vm;
-          }
-        }
+  } else if (x0 < x1) {
+    // ---------------------------------------------------------------- products
+    // Query operand of row 8 r + g, by four-channel groups: two pairs (bf16; f16 for e4m3), or a high and a low digit word
+    // (int8); and what brings the scores of rows 8 r + 2t and + 1 back to size, times log2(e).
+    constexpr bool B16 = CODES == MB_KV_BF16, I8 = CODES == MB_KV_I8;
+    uint32_t qa[RR][QW][2];
+    float q_size[RR][2];
+    // o: channels 16 i + g (0, 1) and + 8 (2, 3) of rows 8 r + 2t and + 1; m, l: of these rows
+    float o[RR][D / 16][4], m[RR][2], l[RR][2];
+    float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and kWeightOne over it
+    uint32_t merges = 0;
+    for (int it = 0;; it++) {
+      const int s = it % STAGES;
+      if (!mbar_wait(&full[s], (it / STAGES) & 1, abort_flag, p.status, kDevTimeoutAttn)) break;
+      const Desc d = desc[s];
+      uint8_t* sk = smem + (size_t)s * S::STAGEB;
+      uint8_t* sv = sk + S::KVB;
+      if (d.q_slot >= 0) {
+        const int rows = min(kRows, p.G - (d.unit % p.q_tiles) * kRows);
 #pragma unroll
         for (int r = 0; r < RR; r++) {
-          float alpha[2];
+          const bool have = g + 8 * r < rows;
+          const uint8_t* src = s_q + d.q_slot * S::QB + (g + 8 * r) * D * 2;
+          uint32_t top = 0;  // largest magnitude's bits: non-negative floats order like integers, NaN last
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float mx = fmaxf(sc[r][e], sc[r][2 + e]);
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            const float mn = mx > m[r][e] + kSlack ? mx : m[r][e];
-            alpha[e] = mn == -INFINITY ? 1.f : ex2_approx(m[r][e] - mn);
-            m[r][e] = mn;
-            l[r][e] *= alpha[e];
-            alpha[e] *= shrink;
-          }
-#pragma unroll
-          for (int i = 0; i < D / 16; i++)
-            o[r][i][0] *= alpha[0], o[r][i][1] *= alpha[1], o[r][i][2] *= alpha[0], o[r][i][3] *= alpha[1];
-        }
-      }
-      vs_a *= v_inv, vs_b *= v_inv;
-      uint32_t w8[RR][2];  // weights as B operand: keys 8 u + 2t and + 1 of row 8 r + g
-#pragma unroll
-      for (int r = 0; r < RR; r++) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const float ref = m[r][e] == -INFINITY ? 0.f : m[r][e];  // nothing but -inf so far: weights 0
-          w[e] = ex2_approx(sc[r][e] - ref), w[2 + e] = ex2_approx(sc[r][2 + e] - ref);
-          l[r][e] += w[e] + w[2 + e];
-        }
-        if (B16) {
-          w8[r][0] = movmatrix(pack_bf16x2(w[0], w[1])), w8[r][1] = movmatrix(pack_bf16x2(w[2], w[3]));
-        } else {
-          const __half2 a = __floats2half2_rn(w[0] * vs_a, w[1] * vs_a), b = __floats2half2_rn(w[2] * vs_b, w[3] * vs_b);
-          w8[r][0] = movmatrix(*(const uint32_t*)&a), w8[r][1] = movmatrix(*(const uint32_t*)&b);
-        }
-      }
-      if (B16) {
-        // values that do not exist may be NaN: zero their rows first (a tile's partial last group only)
-        if (left < 16) {
-          for (int i = lane; i < (16 - left) * (S::ROWB / 16); i += 32) {
-            const int key = key0 + left + i / (S::ROWB / 16);
-            *(uint4*)(sv + S::at(key, (i % (S::ROWB / 16)) * 16)) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        // one instruction: channels 16 i and 16 i + 8 of keys 0-7, then of keys 8-15
-        const int key = key0 + (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) {
-          uint32_t a0, a1, a2, a3;
-          ldmatrix_x4_trans(smem_u32(sv + S::at(key, (2 * i + ((lane >> 3) & 1)) * 16)), a0, a1, a2, a3);
-#pragma unroll
-          for (int r = 0; r < RR; r++) mma16816(o[r][i], a0, a1, a2, a3, w8[r][0], w8[r][1]);
-        }
-      } else {
-        // a weight of 0 silences codes of rows that do not exist, but for e4m3's NaN: those become 0
-#pragma unroll
-        for (int i = 0; i < D / 16; i += 2) {
-          if (WIDE) load_v(i / 2);
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            uint32_t a[4];  // {channels g, g + 8} x {keys 4t, 4t + 1; 4t + 2, 4t + 3}
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              uint32_t x = vw[B16 ? 0 : i / 2][2 * j + e];
-              if (CODES == MB_KV_E4M3 && left < 16)
-                x &= 4 * t >= left ? 0u : left - 4 * t >= 4 ? 0xffffffffu : (1u << (8 * (left - 4 * t))) - 1u;
-              codes_f16<CODES>(x, a[e], a[2 + e]);
+          for (int i = 0; i < QW; i++) {
+            uint2 x = make_uint2(0, 0);
+            if (have) x = *(const uint2*)(src + S::q_channel(i, t) * 2);
+            qa[r][i][0] = x.x, qa[r][i][1] = x.y;
+            if (!B16) {
+              top = max(top, max((x.x << 16) & 0x7fff0000u, (x.y << 16) & 0x7fff0000u));
+              top = max(top, max(x.x & 0x7fff0000u, x.y & 0x7fff0000u));
             }
-#pragma unroll
-            for (int r = 0; r < RR; r++) mma16816_f16(o[r][i + j], a[0], a[1], a[2], a[3], w8[r][0], w8[r][1]);
           }
+          float back = 1.f;
+          if (!B16) {
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            float f;
+            if (I8) {
+              // below 2^-100 the row counts as 0
+              const bool some = top >= 0x0d800000u;
+              f = some ? 32639.f / __uint_as_float(top) : 0.f;
+              back = some ? __uint_as_float(top) / 32639.f : 0.f;
+            } else {  // to [1, 2) by a power of two
+              const int e = min(max((int)(top >> 23), 1), 253);
+              f = __uint_as_float((uint32_t)(254 - e) << 23);
+              back = __uint_as_float((uint32_t)e << 23);
+            }
+            if (top >= 0x7f800000u) f = 0.f, back = __uint_as_float(0x7fc00000u);  // NaN or infinity in the row
+#pragma unroll
+            for (int i = 0; i < QW; i++) {
+              if (I8) {
+                uint32_t h, w;
+                query_digits(make_uint2(qa[r][i][0], qa[r][i][1]), f, h, w);
+                qa[r][i][0] = h, qa[r][i][1] = w;
+              } else {
+                qa[r][i][0] = scaled_f16x2(qa[r][i][0], f), qa[r][i][1] = scaled_f16x2(qa[r][i][1], f);
+              }
+            }
+          }
+          back *= p.scale_log2;
+          q_size[r][0] = __shfl_sync(0xffffffffu, back, 8 * t), q_size[r][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+#pragma unroll
+          for (int i = 0; i < D / 16; i++) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.f;
+          m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.f;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[d.q_slot]);
+        v_ref = v_inv = 0.f;
       }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
-    if (!d.last) continue;
-
-    // the warps' parts together, NR column tiles at a time
-    const int hk = d.unit / p.q_tiles, qt = d.unit - hk * p.q_tiles;
-    const int rows = min(kRows, p.G - qt * kRows), head0 = hk * p.G + qt * kRows;
+      const int key0 = warp * 16;
+      if ((d.groups >> warp) & 1) {
+        const int left = d.left - key0;  // of this warp's 16 keys; > 0
+        // 8-bit values are read ahead of the scores, whose latency hides theirs; where 16 rows leave no registers for
+        // them, when their turn comes
+        uint32_t vw[B16 ? 1 : D / 32][4];
+        auto load_v = [&](int i) {
+          ldmatrix_b8_x2_trans(smem_u32(sv + S::at(key0 + (lane & 15), (2 * i + (lane >> 4)) * 16)), vw[B16 ? 0 : i]);
+        };
+        if (!B16 && !WIDE) {
 #pragma unroll
-    for (int r = 0; r < RR; r++)
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], x);
-        if (g == 0) s_m[warp * kRows + 8 * r + 2 * t + e] = m[r][e], s_l[warp * kRows + 8 * r + 2 * t + e] = l[r][e];
-      }
-    if (lane == 0) s_v[warp] = B16 ? 1.f : v_ref / kWeightOne;
-    bool ok = true;
-    auto meet = [&] {  // of the four warps
-      __syncwarp();
-      if (lane == 0) mbar_arrive(merge_bar);
-      ok = ok && mbar_wait(merge_bar, merges & 1, abort_flag, p.status, kDevTimeoutAttn);
-      merges++;
-    };
-#pragma unroll
-    for (int i0 = 0; i0 < D / 16; i0 += S::NR) {
-#pragma unroll
-      for (int i = 0; i < S::NR; i++)
+          for (int i = 0; i < D / 32; i++) load_v(i);
+        }
+        // scores: sc[r][2 u + e] of key key_of(u, g) and row 8 r + 2t + e
+        const int key_a = S::key_of(0, g), key_b = S::key_of(1, g);
+        float sc[RR][4];
+        int hi[RR][4], lo[RR][4];
 #pragma unroll
         for (int r = 0; r < RR; r++)
 #pragma unroll
-          for (int e = 0; e < 4; e++)
-            s_merge[(warp * S::ROWS + 8 * r + 2 * t + (e & 1)) * S::MERGE_PITCH + i * 16 + g + (e >> 1) * 8] = o[r][i0 + i][e];
-      meet();
-      if (!ok) break;
-      for (int i = threadIdx.x; i < rows * S::NR * 16; i += 32 * kWarps) {
-        const int r = i / (S::NR * 16), col = i % (S::NR * 16), ch = i0 * 16 + col;
-        float top = -INFINITY;
+          for (int e = 0; e < 4; e++) sc[r][e] = 0.f, hi[r][e] = lo[r][e] = 0;
+        constexpr int LB = S::LINEB / 4;  // a lane's bytes of a row in a line
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w * kRows + r]);
-        const float ref1 = top == -INFINITY ? 0.f : top;
-        float acc = 0.f, sum = 0.f;
+        for (int pl = 0; pl < S::PLANES; pl++) {
+          uint32_t wa[LB / 4], wb[LB / 4];
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-          const float f = ex2_approx(s_m[w * kRows + r] - ref1);
-          acc += f * s_v[w] * s_merge[(w * S::ROWS + r) * S::MERGE_PITCH + col];
-          sum += f * s_l[w * kRows + r];
+          for (int i = 0; i < LB / 16; i++) {
+            const uint4 x = *(const uint4*)(sk + S::at(key0 + key_a, pl * 128 + t * LB + i * 16));
+            const uint4 y = *(const uint4*)(sk + S::at(key0 + key_b, pl * 128 + t * LB + i * 16));
+            wa[4 * i] = x.x, wa[4 * i + 1] = x.y, wa[4 * i + 2] = x.z, wa[4 * i + 3] = x.w;
+            wb[4 * i] = y.x, wb[4 * i + 1] = y.y, wb[4 * i + 2] = y.z, wb[4 * i + 3] = y.w;
+          }
+          if (CODES == MB_KV_E4M3) {
+#pragma unroll
+            for (int i = 0; i < LB / 4; i++) {
+              uint32_t a[4];
+              codes_f16<CODES>(wa[i], a[0], a[2]);
+              codes_f16<CODES>(wb[i], a[1], a[3]);
+#pragma unroll
+              for (int r = 0; r < RR; r++) mma16816_f16(sc[r], a[0], a[1], a[2], a[3], qa[r][i][0], qa[r][i][1]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < LB / 8; i++)
+#pragma unroll
+              for (int r = 0; r < RR; r++) {
+                if (B16) {
+                  const uint32_t* q = qa[r][B16 ? pl * 4 + i : 0];
+                  mma16816(sc[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], q[0], q[1]);
+                } else {
+                  const int x = B16 ? 0 : 2 * i, y = B16 ? 0 : 2 * i + 1;
+                  mma16832(hi[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], qa[r][x][0], qa[r][y][0]);
+                  mma16832(lo[r], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], qa[r][x][1], qa[r][y][1]);
+                }
+              }
+          }
         }
-        if (d.slot < 0) {
-          p.out[(int64_t)d.seq * p.ldo + (int64_t)(head0 + r) * D + ch] = __float2bfloat16_rn(acc / sum);
+        // scales of the two keys; those of rows that do not exist may be anything
+        const bool in_a = key_a < left, in_b = key_b < left;
+        float ks_a = 1.f, ks_b = 1.f, vs_a = 1.f, vs_b = 1.f;
+        if (!B16) {
+          const float* scale = (const float*)(sk + 2 * S::KVB) + key0;
+          ks_a = scale[key_a], ks_b = scale[key_b];
+          vs_a = in_a ? scale[kTileKeys + key_a] : 0.f, vs_b = in_b ? scale[kTileKeys + key_b] : 0.f;
+        }
+        // The reference points move (and the output with them) only when a score passes its row's by more than 2^kSlack,
+        // or a value scale the largest so far.
+        bool move = !B16 && fmaxf(vs_a, vs_b) > v_ref;
+#pragma unroll
+        for (int r = 0; r < RR; r++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            if (I8) {  // below 2^30
+              sc[r][e] = (float)(hi[r][e] * 256 + lo[r][e]);
+              sc[r][2 + e] = (float)(hi[r][2 + e] * 256 + lo[r][2 + e]);
+            }
+            sc[r][e] = in_a ? sc[r][e] * (ks_a * q_size[r][e]) : -INFINITY;
+            sc[r][2 + e] = in_b ? sc[r][2 + e] * (ks_b * q_size[r][e]) : -INFINITY;
+            move |= fmaxf(sc[r][e], sc[r][2 + e]) > m[r][e] + kSlack;
+          }
+        if (__any_sync(0xffffffffu, move)) {
+          float shrink = 1.f;
+          if (!B16) {
+            float vm = fmaxf(vs_a, vs_b);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, x));
+            if (vm > v_ref) {  // the same in all lanes
+              shrink = v_ref / vm;
+              v_ref = vm;
+              v_inv = kWeightOne / vm;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < RR; r++) {
+            float alpha[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              float mx = fmaxf(sc[r][e], sc[r][2 + e]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+              const float mn = mx > m[r][e] + kSlack ? mx : m[r][e];
+              alpha[e] = mn == -INFINITY ? 1.f : ex2_approx(m[r][e] - mn);
+              m[r][e] = mn;
+              l[r][e] *= alpha[e];
+              alpha[e] *= shrink;
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+              o[r][i][0] *= alpha[0], o[r][i][1] *= alpha[1], o[r][i][2] *= alpha[0], o[r][i][3] *= alpha[1];
+          }
+        }
+        vs_a *= v_inv, vs_b *= v_inv;
+        uint32_t w8[RR][2];  // weights as B operand: keys 8 u + 2t and + 1 of row 8 r + g
+#pragma unroll
+        for (int r = 0; r < RR; r++) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float ref = m[r][e] == -INFINITY ? 0.f : m[r][e];  // nothing but -inf so far: weights 0
+            w[e] = ex2_approx(sc[r][e] - ref), w[2 + e] = ex2_approx(sc[r][2 + e] - ref);
+            l[r][e] += w[e] + w[2 + e];
+          }
+          if (B16) {
+            w8[r][0] = movmatrix(pack_bf16x2(w[0], w[1])), w8[r][1] = movmatrix(pack_bf16x2(w[2], w[3]));
+          } else {
+            const __half2 a = __floats2half2_rn(w[0] * vs_a, w[1] * vs_a), b = __floats2half2_rn(w[2] * vs_b, w[3] * vs_b);
+            w8[r][0] = movmatrix(*(const uint32_t*)&a), w8[r][1] = movmatrix(*(const uint32_t*)&b);
+          }
+        }
+        if (B16) {
+          // values that do not exist may be NaN: zero their rows first (a tile's partial last group only)
+          if (left < 16) {
+            for (int i = lane; i < (16 - left) * (S::ROWB / 16); i += 32) {
+              const int key = key0 + left + i / (S::ROWB / 16);
+              *(uint4*)(sv + S::at(key, (i % (S::ROWB / 16)) * 16)) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          // one instruction: channels 16 i and 16 i + 8 of keys 0-7, then of keys 8-15
+          const int key = key0 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+          for (int i = 0; i < D / 16; i++) {
+            uint32_t a0, a1, a2, a3;
+            ldmatrix_x4_trans(smem_u32(sv + S::at(key, (2 * i + ((lane >> 3) & 1)) * 16)), a0, a1, a2, a3);
+#pragma unroll
+            for (int r = 0; r < RR; r++) mma16816(o[r][i], a0, a1, a2, a3, w8[r][0], w8[r][1]);
+          }
         } else {
-          p.part_o[((int64_t)d.slot * kRows + r) * D + ch] = acc;
-          if (ch == 0) {
-            p.part_ml[(int64_t)d.slot * 2 * kRows + r] = top;
-            p.part_ml[(int64_t)d.slot * 2 * kRows + kRows + r] = sum;
+          // a weight of 0 silences codes of rows that do not exist, but for e4m3's NaN: those become 0
+#pragma unroll
+          for (int i = 0; i < D / 16; i += 2) {
+            if (WIDE) load_v(i / 2);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              uint32_t a[4];  // {channels g, g + 8} x {keys 4t, 4t + 1; 4t + 2, 4t + 3}
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                uint32_t x = vw[B16 ? 0 : i / 2][2 * j + e];
+                if (CODES == MB_KV_E4M3 && left < 16)
+                  x &= 4 * t >= left ? 0u : left - 4 * t >= 4 ? 0xffffffffu : (1u << (8 * (left - 4 * t))) - 1u;
+                codes_f16<CODES>(x, a[e], a[2 + e]);
+              }
+#pragma unroll
+              for (int r = 0; r < RR; r++) mma16816_f16(o[r][i + j], a[0], a[1], a[2], a[3], w8[r][0], w8[r][1]);
+            }
           }
         }
       }
-      meet();
-      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+      if (!d.last) continue;
+
+      // the warps' parts together, NR column tiles at a time
+      const int hk = d.unit / p.q_tiles, qt = d.unit - hk * p.q_tiles;
+      const int rows = min(kRows, p.G - qt * kRows), head0 = hk * p.G + qt * kRows;
+#pragma unroll
+      for (int r = 0; r < RR; r++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], x);
+          if (g == 0) s_m[warp * kRows + 8 * r + 2 * t + e] = m[r][e], s_l[warp * kRows + 8 * r + 2 * t + e] = l[r][e];
+        }
+      if (lane == 0) s_v[warp] = B16 ? 1.f : v_ref / kWeightOne;
+      bool ok = true;
+      auto meet = [&] {  // of the four warps
+        __syncwarp();
+        if (lane == 0) mbar_arrive(merge_bar);
+        ok = ok && mbar_wait(merge_bar, merges & 1, abort_flag, p.status, kDevTimeoutAttn);
+        merges++;
+      };
+#pragma unroll
+      for (int i0 = 0; i0 < D / 16; i0 += S::NR) {
+#pragma unroll
+        for (int i = 0; i < S::NR; i++)
+#pragma unroll
+          for (int r = 0; r < RR; r++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              s_merge[(warp * S::ROWS + 8 * r + 2 * t + (e & 1)) * S::MERGE_PITCH + i * 16 + g + (e >> 1) * 8] = o[r][i0 + i][e];
+        meet();
+        if (!ok) break;
+        for (int i = threadIdx.x; i < rows * S::NR * 16; i += 32 * kWarps) {
+          const int r = i / (S::NR * 16), col = i % (S::NR * 16), ch = i0 * 16 + col;
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w * kRows + r]);
+          const float ref1 = top == -INFINITY ? 0.f : top;
+          float acc = 0.f, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; w++) {
+            const float f = ex2_approx(s_m[w * kRows + r] - ref1);
+            acc += f * s_v[w] * s_merge[(w * S::ROWS + r) * S::MERGE_PITCH + col];
+            sum += f * s_l[w * kRows + r];
+          }
+          if (CLUSTER) {
+            part[r * D + ch] = acc;
+            if (ch == 0) part[S::ROWS * D + r] = top, part[S::ROWS * D + S::ROWS + r] = sum;
+          } else if (d.slot < 0) {
+            p.out[(int64_t)d.seq * p.ldo + (int64_t)(head0 + r) * D + ch] = __float2bfloat16_rn(acc / sum);
+          } else {
+            p.part_o[((int64_t)d.slot * kRows + r) * D + ch] = acc;
+            if (ch == 0) {
+              p.part_ml[(int64_t)d.slot * 2 * kRows + r] = top;
+              p.part_ml[(int64_t)d.slot * 2 * kRows + kRows + r] = sum;
+            }
+          }
+        }
+        meet();
+        if (!ok) break;
+      }
+      if (!ok || d.end) break;
     }
-    if (!ok) break;
+  }
+
+  if constexpr (CLUSTER) {
+    // the unit's parts lie in its blocks' memory; each block joins every eighth row
+    __syncwarp();
+    cluster_sync();
+    const int hk = unit / p.q_tiles, qt = unit - hk * p.q_tiles;
+    const int rows = min(kRows, p.G - qt * kRows), head0 = hk * p.G + qt * kRows;
+    auto has_tiles = [&](int k) { return nt * k / kCluster < nt * (k + 1) / kCluster; };
+    for (int r = rank; r < rows; r += kCluster)
+      for (int d = threadIdx.x; d < D; d += kThreads) {
+        float top = -INFINITY, m[kCluster], acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kCluster; k++) {
+          m[k] = has_tiles(k) ? ld_cluster(part + S::ROWS * D + r, k) : -INFINITY;
+          top = fmaxf(top, m[k]);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < kCluster; k++)
+          if (has_tiles(k)) {
+            const float f = ex2_approx(m[k] - ref);
+            acc += f * ld_cluster(part + r * D + d, k);
+            sum += f * ld_cluster(part + S::ROWS * D + S::ROWS + r, k);
+          }
+        p.out[(int64_t)b * p.ldo + (int64_t)(head0 + r) * D + d] = __float2bfloat16_rn(nt > 0 ? acc / sum : 0.f);
+      }
+    __syncwarp();
+    cluster_sync();  // no block's memory goes while another reads it
   }
 }
 
@@ -750,8 +822,8 @@ Layout layout(int n_seqs, int H, int H_kv, int D) {
   return a;
 }
 
-template <int CODES, int D, bool WIDE>
-cudaError_t launch_attention(const Params& p, cudaStream_t st) {
+template <int CODES, int D, bool WIDE, bool CLUSTER>
+cudaError_t launch_attention(const Params& p, int64_t units, cudaStream_t st) {
   using S = Shape<CODES, D, WIDE>;
   CUtensorMap tk, tv;
   // lines of 128 bytes: rows of 256 bytes as two columns of boxes, rows of 64 two to a line
@@ -761,25 +833,40 @@ cudaError_t launch_attention(const Params& p, cudaStream_t st) {
     if (!make_tmap_2d(i ? &tv : &tk, i ? p.c.v : p.c.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, inner, rows, inner, 128,
                       S::GROUPB / 128, CU_TENSOR_MAP_SWIZZLE_128B))
       return cudaErrorInvalidValue;
+  auto kernel = k_attention_paged<CODES, D, WIDE, CLUSTER>;
   static int attr_done[64];
   int dev = 0;
   cudaGetDevice(&dev);
   if (!attr_done[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(k_attention_paged<CODES, D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)S::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
     if (e != cudaSuccess) return e;
     attr_done[dev & 63] = 1;
   }
-  k_attention_paged<CODES, D, WIDE><<<(unsigned)(num_sms() * S::BLOCKS), kThreads, S::kSmem, st>>>(tk, tv, p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(CLUSTER ? units * kCluster : num_sms() * S::BLOCKS));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kCluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CLUSTER ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, tk, tv, p);
 }
 
-template <int CODES, int D>
+template <int CODES, int D, bool WIDE>
 cudaError_t launch(const Params& p, int64_t units, cudaStream_t st) {
-  cudaError_t e = p.G > 8 ? launch_attention<CODES, D, true>(p, st) : launch_attention<CODES, D, false>(p, st);
-  if (e != cudaSuccess) return e;
+  using S = Shape<CODES, D, WIDE>;
+  const int64_t keys = (int64_t)p.table_width << p.c.page_log2;  // at most, of a sequence
+  // Few units of a few tiles a block: their parts meet inside a cluster (28/4 heads, 700 positions: 8.2 us against 10.2
+  // with a second launch). More or longer ones want all SMs, and the even cut.
+  if (keys > kTileKeys && keys <= 8 * kCluster * kTileKeys && units * kCluster <= (int64_t)num_sms() * S::BLOCKS)
+    return launch_attention<CODES, D, WIDE, true>(p, units, st);
+  cudaError_t e = launch_attention<CODES, D, WIDE, false>(p, units, st);
   // a unit that fits a tile is never split
-  if (((int64_t)p.table_width << p.c.page_log2) <= kTileKeys) return cudaSuccess;
+  if (e != cudaSuccess || keys <= kTileKeys) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)units, (unsigned)(p.G < kRows ? p.G : kRows));
   cfg.blockDim = dim3(32 * kJoinWarps);
@@ -790,6 +877,11 @@ cudaError_t launch(const Params& p, int64_t units, cudaStream_t st) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k_join<D>, p);
+}
+
+template <int CODES, int D>
+cudaError_t launch(const Params& p, int64_t units, cudaStream_t st) {
+  return p.G > 8 ? launch<CODES, D, true>(p, units, st) : launch<CODES, D, false>(p, units, st);
 }
 
 }  // namespace paged

@@ -395,6 +395,23 @@ def test_paged_splits(cuda, dtype, lengths):
         close(out[b:b + 1], *U.attention64(q[b:b + 1], k, v, keep, half_weights=dtype != torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", [(4, 1, 128), (12, 4, 64), (40, 2, 128)])
+def test_paged_short_and_long_tables(cuda, dtype, H, Hkv, D):
+    """The same sequences under a table of few pages, whose parts meet in a cluster, and one of many, which is cut over
+    all SMs; 1 to more tiles than a cluster has blocks, and none."""
+    for lengths in ([700], [0, 1, 4000], [64, 65], [512, 513, 1100], [0]):
+        cache, pages = filled(dtype, lengths, 16, Hkv, D, 150)
+        q = rand((len(lengths), H, D), 151, 1.5)
+        wide = torch.full((len(lengths), 300), -1, dtype=torch.int32, device="cuda")
+        wide[:, :pages.table.shape[1]] = pages.table
+        for table in (pages.table, wide):
+            out = mb.attention_paged(q, cache, table, ints(lengths))
+            check_paged(q, cache, pages, lengths, out)
+            assert torch.equal(out, mb.attention_paged(q, cache, table, ints(lengths)))
+    assert mb.device_status() == 0
+
+
 def test_paged_layouts_scale_and_padding(cuda):
     """Strided q and out, a table wider than the pages, lengths behind the table cut to it, negative lengths, scales."""
     lengths = [100, 7, 48]
