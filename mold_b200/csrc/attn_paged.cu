@@ -860,8 +860,9 @@ template <int CODES, int D, bool WIDE>
 cudaError_t launch(const Params& p, int64_t units, cudaStream_t st) {
   using S = Shape<CODES, D, WIDE>;
   const int64_t keys = (int64_t)p.table_width << p.c.page_log2;  // at most, of a sequence
-  // Few units of a few tiles a block: their parts meet inside a cluster (28/4 heads, 700 positions: 8.2 us against 10.2
-  // with a second launch). More or longer ones want all SMs, and the even cut.
+  // Few units of a few tiles a block: their parts meet inside a cluster instead of in a second launch. bf16, in a graph:
+  // one sequence of 700, 28/4 heads, 7.1 us against 10.0; eight of 4000 13.6 against 16.3; one of 4000, 32/8 heads, 11.8
+  // against 11.5, where 64 blocks leave SMs idle. More or longer ones want all SMs, and the even cut.
   if (keys > kTileKeys && keys <= 8 * kCluster * kTileKeys && units * kCluster <= (int64_t)num_sms() * S::BLOCKS)
     return launch_attention<CODES, D, WIDE, true>(p, units, st);
   cudaError_t e = launch_attention<CODES, D, WIDE, false>(p, units, st);

@@ -17,19 +17,34 @@ namespace kv {
 constexpr int kRows = 2;   // rows a group handles
 constexpr int kHalves = 2;  // 16-byte pieces of a bf16 row that a thread holds, half a row apart
 
-// The sequence whose rows hold t: the last b with cu[b] <= t. All lanes of the warp with the same t; 32 entries a step.
-// Whatever cu holds, b is in [0, n).
-MB_DEV int seq_of(const int32_t* cu, int n, int64_t t) {
+// The sequence whose rows hold t: the last b with cu[b] <= t, its rows [c0, c1), and its entry of `per_seq` (NULL: 0). All
+// lanes of the warp with the same t; 32 entries a step, and the last step's loads serve for all of it, since each load
+// that waits for another costs as much as the row's own. Whatever cu holds, b is in [0, n).
+struct Span {
+  int b;
+  int64_t c0, c1;
+  int value;
+};
+MB_DEV Span seq_of(const int32_t* cu, const int32_t* per_seq, int n, int64_t t) {
   const int lane = threadIdx.x & 31;
   int lo = 0;
-  while (n > 1) {
+  while (n > 32) {
     const int step = (n + 31) >> 5, at = lane * step;
     const unsigned le = __ballot_sync(0xffffffffu, at < n && __ldg(cu + lo + (at < n ? at : 0)) <= t);
     const int k = max(__popc(le), 1) - 1;  // le is a run of ones from bit 0
     lo += k * step;
     n = min(step, n - k * step);
   }
-  return lo;
+  const int edge = lane <= n ? __ldg(cu + lo + lane) : 0;
+  const int value = per_seq && lane < n ? __ldg(per_seq + lo + lane) : 0;
+  const int k = max(__popc(__ballot_sync(0xffffffffu, lane < n && edge <= t)), 1) - 1;
+  Span s;
+  s.b = lo + k;
+  s.c0 = __shfl_sync(0xffffffffu, edge, k);
+  s.c1 = __shfl_sync(0xffffffffu, edge, (k + 1) & 31);
+  if (k == 31) s.c1 = __ldg(cu + lo + 32);
+  s.value = __shfl_sync(0xffffffffu, value, k);
+  return s;
 }
 
 MB_DEV uint64_t pack2(float a, float b) {
@@ -171,8 +186,8 @@ __global__ void __launch_bounds__(256) k_kv_write(const WriteParams p) {
   }
   // places in the cache, while the rows are on their way
   int64_t dst[kRows], base = -1;
-  int b = p.cu ? seq_of(p.cu, p.n_seqs, first.t) : 0;
-  int64_t c1 = p.cu ? (int64_t)__ldg(p.cu + b + 1) : 0;
+  Span seq = {0, 0, 0, 0};
+  if (p.cu) seq = seq_of(p.cu, p.lens, p.n_seqs, first.t);
   w = own;
   bool moved = true;
 #pragma unroll
@@ -182,13 +197,16 @@ __global__ void __launch_bounds__(256) k_kv_write(const WriteParams p) {
       if (w.t < p.n_tokens) {
         int64_t pos;
         if (p.cu) {
-          while (w.t >= c1 && b + 1 < p.n_seqs) c1 = __ldg(p.cu + ++b + 1);
-          pos = w.t < c1 && w.t >= __ldg(p.cu + b) ? (int64_t)__ldg(p.lens + b) - (c1 - w.t) : -1;
+          while (w.t >= seq.c1 && seq.b + 1 < p.n_seqs) {
+            seq.b++, seq.c0 = seq.c1, seq.c1 = __ldg(p.cu + seq.b + 1);
+            seq.value = __ldg(p.lens + seq.b);
+          }
+          pos = w.t >= seq.c0 && w.t < seq.c1 ? seq.value - (seq.c1 - w.t) : -1;
         } else {
-          b = (int)w.t;
-          pos = (int64_t)__ldg(p.lens + b) - 1;
+          seq.b = (int)w.t;
+          pos = (int64_t)__ldg(p.lens + seq.b) - 1;
         }
-        if (pos >= 0) base = row_of(p.c, p.table + (int64_t)b * p.ld_table, p.table_width, pos, 0, p.status);
+        if (pos >= 0) base = row_of(p.c, p.table + (int64_t)seq.b * p.ld_table, p.table_width, pos, 0, p.status);
       }
     }
     dst[i] = base < 0 ? -1 : base + ((int64_t)w.h << p.c.page_log2);
@@ -292,8 +310,8 @@ __global__ void __launch_bounds__(256) k_kv_read(const ReadParams p) {
   const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (SIDE * kRows);
   if (row0 >= p.n_tokens * p.c.heads) return;
   const Walk first(row0, p.c.heads);
-  int b = seq_of(p.cu, p.n_seqs, first.t);
-  int64_t c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1), base = -1;
+  Span seq = seq_of(p.cu, nullptr, p.n_seqs, first.t);
+  int64_t base = -1;
   Held<CODES> kx[kRows], vx[kRows];
   bool mine[kRows], moved = true, own = false;  // rows that are some sequence's
   Walk w = first;
@@ -305,9 +323,9 @@ __global__ void __launch_bounds__(256) k_kv_read(const ReadParams p) {
       base = -1;
       own = false;
       if (w.t < p.n_tokens) {
-        while (w.t >= c1 && b + 1 < p.n_seqs) b++, c0 = c1, c1 = __ldg(p.cu + b + 1);
-        own = w.t >= c0 && w.t < c1;
-        if (own) base = row_of(p.c, p.table + (int64_t)b * p.ld_table, p.table_width, w.t - c0, 0, p.status);
+        while (w.t >= seq.c1 && seq.b + 1 < p.n_seqs) seq.b++, seq.c0 = seq.c1, seq.c1 = __ldg(p.cu + seq.b + 1);
+        own = w.t >= seq.c0 && w.t < seq.c1;
+        if (own) base = row_of(p.c, p.table + (int64_t)seq.b * p.ld_table, p.table_width, w.t - seq.c0, 0, p.status);
       }
     }
     mine[i] = own;
