@@ -2,9 +2,11 @@
 // one f32 scale for each row of head_dim values) and read back.
 //
 // A group of head_dim / 16 threads owns a (token, head) row of k and the same row of v, two times 16 bytes
-// of bf16 a thread; a warp walks kRows rows of each group, so that the search for the sequence is made once
-// and every load of the warp is in flight before the first is used. Bound by HBM, with little to spare for
-// instructions: hence packed f32 arithmetic and no integer conversions or divisions.
+// of bf16 a thread; the groups of a warp work on neighbouring rows and search for the sequence together,
+// while the rows are on their way. Bound by HBM, with little to spare for instructions: hence packed f32
+// arithmetic and no integer conversions or divisions (with them: 61 to 68 % of the issue slots, 55 us
+// where it is 41 for 11k rows of 8 x 128 written and 25k read, int8). More rows a thread or larger blocks
+// lose (2 rows: 41.2, 4: 48 us; a generation step 6.1 and 9.6 against 4.8 us).
 #include <string>
 
 #include "common.cuh"
@@ -14,7 +16,7 @@
 namespace mb {
 namespace kv {
 
-constexpr int kRows = 2;   // rows a group handles
+constexpr int kThreads = 128;
 constexpr int kHalves = 2;  // 16-byte pieces of a bf16 row that a thread holds, half a row apart
 
 // The sequence whose rows hold t: the last b with cu[b] <= t, its rows [c0, c1), and its entry of `per_seq` (NULL: 0). All
@@ -69,21 +71,18 @@ MB_DEV uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// The row of a warp's first group, and a step from it to the next of a group's rows.
-struct Walk {
-  int64_t t;
-  int h, heads;
-  MB_DEV Walk(int64_t row, int heads_) : heads(heads_) {
-    t = row < (1LL << 32) ? (int64_t)((uint32_t)row / (uint32_t)heads_) : row / heads_;
-    h = (int)(row - t * heads_);
+// Token and head of a row.
+MB_DEV void split_row(int64_t row, int heads, int64_t& t, int& h) {
+  t = row < (1LL << 32) ? (int64_t)((uint32_t)row / (uint32_t)heads) : row / heads;
+  h = (int)(row - t * heads);
+}
+// On to the sequence that holds t, at or behind the present one.
+MB_DEV void advance(Span& s, const int32_t* cu, const int32_t* per_seq, int n, int64_t t) {
+  while (t >= s.c1 && s.b + 1 < n) {
+    s.b++, s.c0 = s.c1, s.c1 = __ldg(cu + s.b + 1);
+    if (per_seq) s.value = __ldg(per_seq + s.b);
   }
-  MB_DEV bool next(int by) {  // whether the token changed
-    h += by;
-    if (h < heads) return false;
-    while (h >= heads) h -= heads, t++;
-    return true;
-  }
-};
+}
 
 struct WriteParams {
   Cache c;
@@ -163,78 +162,57 @@ MB_DEV void encode_row(const uint4 (&x)[kHalves], uint2 (&out)[kHalves], float& 
 }
 
 template <int CODES, int D>
-__global__ void __launch_bounds__(256) k_kv_write(const WriteParams p) {
+__global__ void __launch_bounds__(kThreads) k_kv_write(const WriteParams p) {
   constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
-  const int lane = threadIdx.x % GROUP, side = (threadIdx.x & 31) / GROUP;
-  const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (SIDE * kRows);  // the warp's
+  const int lane = threadIdx.x % GROUP;
+  const int64_t row0 = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * SIDE;  // the warp's first
   if (row0 >= p.n_tokens * p.c.heads) return;
-  const Walk first(row0, p.c.heads);
-  Walk w = first;
-  w.next(side);
-  const Walk own = w;
-  uint4 kx[kRows][kHalves], vx[kRows][kHalves];
+  int64_t t0, t;
+  int h0, h;
+  split_row(row0, p.c.heads, t0, h0);
+  split_row(row0 + (threadIdx.x & 31) / GROUP, p.c.heads, t, h);
+  const bool here = t < p.n_tokens;
+  uint4 kx[kHalves], vx[kHalves];
 #pragma unroll
-  for (int i = 0; i < kRows; i++) {
-    const uint4* ks = (const uint4*)(p.k + w.t * p.ldk + w.h * D) + lane;
-    const uint4* vs = (const uint4*)(p.v + w.t * p.ldv + w.h * D) + lane;
-#pragma unroll
-    for (int j = 0; j < kHalves; j++) {
-      kx[i][j] = vx[i][j] = make_uint4(0, 0, 0, 0);
-      if (w.t < p.n_tokens) kx[i][j] = ld_stream(ks + j * GROUP), vx[i][j] = ld_stream(vs + j * GROUP);
+  for (int j = 0; j < kHalves; j++) {
+    kx[j] = vx[j] = make_uint4(0, 0, 0, 0);
+    if (here) {
+      kx[j] = ld_stream((const uint4*)(p.k + t * p.ldk + h * D) + j * GROUP + lane);
+      vx[j] = ld_stream((const uint4*)(p.v + t * p.ldv + h * D) + j * GROUP + lane);
     }
-    w.next(SIDE);
   }
-  // places in the cache, while the rows are on their way
-  int64_t dst[kRows], base = -1;
-  Span seq = {0, 0, 0, 0};
-  if (p.cu) seq = seq_of(p.cu, p.lens, p.n_seqs, first.t);
-  w = own;
-  bool moved = true;
-#pragma unroll
-  for (int i = 0; i < kRows; i++) {
-    if (moved) {
-      base = -1;
-      if (w.t < p.n_tokens) {
-        int64_t pos;
-        if (p.cu) {
-          while (w.t >= seq.c1 && seq.b + 1 < p.n_seqs) {
-            seq.b++, seq.c0 = seq.c1, seq.c1 = __ldg(p.cu + seq.b + 1);
-            seq.value = __ldg(p.lens + seq.b);
-          }
-          pos = w.t >= seq.c0 && w.t < seq.c1 ? seq.value - (seq.c1 - w.t) : -1;
-        } else {
-          seq.b = (int)w.t;
-          pos = (int64_t)__ldg(p.lens + seq.b) - 1;
-        }
-        if (pos >= 0) base = row_of(p.c, p.table + (int64_t)seq.b * p.ld_table, p.table_width, pos, 0, p.status);
-      }
+  int64_t dst = -1, pos = -1;
+  Span seq = {(int)t, 0, 0, 0};
+  if (p.cu) {
+    seq = seq_of(p.cu, p.lens, p.n_seqs, t0);
+    if (here) {
+      advance(seq, p.cu, p.lens, p.n_seqs, t);
+      if (t >= seq.c0 && t < seq.c1) pos = seq.value - (seq.c1 - t);
     }
-    dst[i] = base < 0 ? -1 : base + ((int64_t)w.h << p.c.page_log2);
-    moved = w.next(SIDE);
+  } else if (here) {
+    pos = (int64_t)__ldg(p.lens + seq.b) - 1;
   }
+  if (pos >= 0) dst = row_of(p.c, p.table + (int64_t)seq.b * p.ld_table, p.table_width, pos, h, p.status);
+  if (CODES == MB_KV_BF16) {
+    if (dst >= 0)
 #pragma unroll
-  for (int i = 0; i < kRows; i++) {
-    if (CODES == MB_KV_BF16) {
-      if (dst[i] >= 0)
-#pragma unroll
-        for (int j = 0; j < kHalves; j++) {
-          ((uint4*)p.c.k)[dst[i] * (D / 8) + j * GROUP + lane] = kx[i][j];
-          ((uint4*)p.c.v)[dst[i] * (D / 8) + j * GROUP + lane] = vx[i][j];
-        }
-    } else {  // shuffles inside: every lane
-      float ks, vs;
-      uint2 kc[kHalves], vc[kHalves];
-      encode_row<CODES, GROUP>(kx[i], kc, ks);
-      encode_row<CODES, GROUP>(vx[i], vc, vs);
-      if (dst[i] >= 0) {
-#pragma unroll
-        for (int j = 0; j < kHalves; j++) {
-          ((uint2*)p.c.k)[dst[i] * (D / 8) + j * GROUP + lane] = kc[j];
-          ((uint2*)p.c.v)[dst[i] * (D / 8) + j * GROUP + lane] = vc[j];
-        }
-        if (lane == 0) p.c.k_scale[dst[i]] = ks;
-        if (lane == 1) p.c.v_scale[dst[i]] = vs;
+      for (int j = 0; j < kHalves; j++) {
+        ((uint4*)p.c.k)[dst * (D / 8) + j * GROUP + lane] = kx[j];
+        ((uint4*)p.c.v)[dst * (D / 8) + j * GROUP + lane] = vx[j];
       }
+  } else {  // shuffles inside: every lane
+    float ks, vs;
+    uint2 kc[kHalves], vc[kHalves];
+    encode_row<CODES, GROUP>(kx, kc, ks);
+    encode_row<CODES, GROUP>(vx, vc, vs);
+    if (dst >= 0) {
+#pragma unroll
+      for (int j = 0; j < kHalves; j++) {
+        ((uint2*)p.c.k)[dst * (D / 8) + j * GROUP + lane] = kc[j];
+        ((uint2*)p.c.v)[dst * (D / 8) + j * GROUP + lane] = vc[j];
+      }
+      if (lane == 0) p.c.k_scale[dst] = ks;
+      if (lane == 1) p.c.v_scale[dst] = vs;
     }
   }
 }
@@ -304,55 +282,33 @@ MB_DEV uint4 decode_row(const Held<CODES>& r, int j) {
 }
 
 template <int CODES, int D>
-__global__ void __launch_bounds__(256) k_kv_read(const ReadParams p) {
+__global__ void __launch_bounds__(kThreads) k_kv_read(const ReadParams p) {
   constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
-  const int lane = threadIdx.x % GROUP, side = (threadIdx.x & 31) / GROUP;
-  const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (SIDE * kRows);
+  const int lane = threadIdx.x % GROUP;
+  const int64_t row0 = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * SIDE;
   if (row0 >= p.n_tokens * p.c.heads) return;
-  const Walk first(row0, p.c.heads);
-  Span seq = seq_of(p.cu, nullptr, p.n_seqs, first.t);
-  int64_t base = -1;
-  Held<CODES> kx[kRows], vx[kRows];
-  bool mine[kRows], moved = true, own = false;  // rows that are some sequence's
-  Walk w = first;
-  w.next(side);
-  const Walk begin = w;
+  int64_t t0, t;
+  int h0, h;
+  split_row(row0, p.c.heads, t0, h0);
+  split_row(row0 + (threadIdx.x & 31) / GROUP, p.c.heads, t, h);
+  Span seq = seq_of(p.cu, nullptr, p.n_seqs, t0);
+  if (t >= p.n_tokens) return;
+  advance(seq, p.cu, nullptr, p.n_seqs, t);
+  if (t < seq.c0 || t >= seq.c1) return;  // nobody's row
+  const int64_t src = row_of(p.c, p.table + (int64_t)seq.b * p.ld_table, p.table_width, t - seq.c0, h, p.status);
+  Held<CODES> kx, vx;
+  load_row<CODES, D>(kx, p.c.k, p.c.k_scale, src, lane);
+  load_row<CODES, D>(vx, p.c.v, p.c.v_scale, src, lane);
 #pragma unroll
-  for (int i = 0; i < kRows; i++) {
-    if (moved) {
-      base = -1;
-      own = false;
-      if (w.t < p.n_tokens) {
-        while (w.t >= seq.c1 && seq.b + 1 < p.n_seqs) seq.b++, seq.c0 = seq.c1, seq.c1 = __ldg(p.cu + seq.b + 1);
-        own = w.t >= seq.c0 && w.t < seq.c1;
-        if (own) base = row_of(p.c, p.table + (int64_t)seq.b * p.ld_table, p.table_width, w.t - seq.c0, 0, p.status);
-      }
-    }
-    mine[i] = own;
-    const int64_t src = base < 0 ? -1 : base + ((int64_t)w.h << p.c.page_log2);
-    load_row<CODES, D>(kx[i], p.c.k, p.c.k_scale, src, lane);
-    load_row<CODES, D>(vx[i], p.c.v, p.c.v_scale, src, lane);
-    moved = w.next(SIDE);
-  }
-  w = begin;
-#pragma unroll
-  for (int i = 0; i < kRows; i++) {
-    if (mine[i]) {
-      uint4* kd = (uint4*)(p.k + w.t * p.ldk + w.h * D) + lane;
-      uint4* vd = (uint4*)(p.v + w.t * p.ldv + w.h * D) + lane;
-#pragma unroll
-      for (int j = 0; j < kHalves; j++) {
-        kd[j * GROUP] = decode_row<CODES>(kx[i], j);
-        vd[j * GROUP] = decode_row<CODES>(vx[i], j);
-      }
-    }
-    w.next(SIDE);
+  for (int j = 0; j < kHalves; j++) {
+    *((uint4*)(p.k + t * p.ldk + h * D) + j * GROUP + lane) = decode_row<CODES>(kx, j);
+    *((uint4*)(p.v + t * p.ldv + h * D) + j * GROUP + lane) = decode_row<CODES>(vx, j);
   }
 }
 
-// Blocks of 8 warps for the rows of n_tokens tokens
+// Blocks for the rows of n_tokens tokens
 inline int64_t blocks_of(int64_t n_tokens, const mb_kv_cache* c) {
-  const int64_t per_block = 256 / (c->head_dim / 16) * kRows;
+  const int64_t per_block = kThreads / (c->head_dim / 16);
   return (n_tokens * c->n_kv_heads + per_block - 1) / per_block;
 }
 
@@ -439,7 +395,7 @@ mb_status mb_kv_write(const mb_kv_cache* cache, const void* k, int64_t ldk, cons
   const kv::WriteParams p = {device_cache(cache), (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, ldk, ldv, n_tokens,
                              cu, kv_lens, table, ld_table, table_width, n_seqs, device_status_ptr()};
   MB_CUDA(kv::dispatch(cache, [&](auto codes, auto dim) {
-    kv::k_kv_write<decltype(codes)::value, decltype(dim)::value><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(p);
+    kv::k_kv_write<decltype(codes)::value, decltype(dim)::value><<<(unsigned)blocks, kv::kThreads, 0, (cudaStream_t)stream>>>(p);
     return cudaGetLastError();
   }));
   return MB_OK;
@@ -463,7 +419,7 @@ mb_status mb_kv_read(const mb_kv_cache* cache, const int32_t* cu, const int32_t*
   const kv::ReadParams p = {device_cache(cache), cu, table, ld_table, table_width, n_seqs, n_tokens,
                             (__nv_bfloat16*)k, (__nv_bfloat16*)v, ldk, ldv, device_status_ptr()};
   MB_CUDA(kv::dispatch(cache, [&](auto codes, auto dim) {
-    kv::k_kv_read<decltype(codes)::value, decltype(dim)::value><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(p);
+    kv::k_kv_read<decltype(codes)::value, decltype(dim)::value><<<(unsigned)blocks, kv::kThreads, 0, (cudaStream_t)stream>>>(p);
     return cudaGetLastError();
   }));
   return MB_OK;
