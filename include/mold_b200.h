@@ -450,8 +450,8 @@ MB_API mb_status mb_attention_varlen(const void* q, int64_t ldq, const void* k, 
 
 /* K12. Append to the cache: sequence b's rows of k, v (bf16 [n_tokens, n_kv_heads, head_dim]) go
  * to its last positions, kv_lens[b] - m .. kv_lens[b] - 1 (kv_lens: device int32, the lengths
- * after the call). cu NULL: one row each (n_tokens == n_seqs); a sequence with kv_lens[b] <= 0
- * is passed over. MB_KV_BF16 keeps the values. The 8-bit types keep for each row of head_dim
+ * after the call). cu NULL: one row each (n_tokens == n_seqs). Rows that would come before
+ * position 0 are passed over (kv_lens[b] <= 0: a sequence of a padded batch). MB_KV_BF16 keeps the values. The 8-bit types keep for each row of head_dim
  * values x the scale s = max|x| / T and the codes c nearest to x * (T / max|x|), ties to even
  * (scale, inverse and product rounded to f32; T = 127 or 448), standing for c * s. A row whose
  * largest magnitude is below 2^-100 is stored as zeros; one with a NaN or infinity reads back

@@ -459,7 +459,7 @@ class KVCache:
     def write(self, k, v, table, kv_lens, cu=None):
         """Append rows k, v (bf16 [T, n_kv_heads, head_dim]): sequence b's rows [cu[b], cu[b+1]) become its last
         positions, kv_lens[b] (int32, the length after the call) at their end. Without cu, row b is sequence b's one
-        new position, and a sequence with kv_lens[b] <= 0 gets none."""
+        new position. Rows that would come before position 0 are passed over (kv_lens[b] <= 0 in a padded batch)."""
         dev = _ready(self.k, k, v, table, kv_lens, cu)
         k, k_ptr, ldk, rows = self._rows(k, "k")
         v, v_ptr, ldv, v_rows = self._rows(v, "v")

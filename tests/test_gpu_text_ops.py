@@ -312,6 +312,25 @@ def test_write_one_token_each(cuda):
     assert mb.device_status() == 0
 
 
+def test_write_before_position_zero_and_unowned_rows(cuda):
+    """A length shorter than the rows of its sequence keeps the last ones; rows before the first and behind the last
+    sequence belong to nobody; offsets that do not begin at 0."""
+    cache, pages = make(torch.int8, [40, 40], 16, 2, 64)
+    k, v = rand((70, 2, 64), 45), rand((70, 2, 64), 46)
+    cache.write(k, v, pages.table, ints([10, 33]), cu=ints([3, 20, 60]))
+    assert mb.device_status() == 0
+    n = [10, 33]
+    for b, first in ((0, 10), (1, 27)):  # sequence 0: rows 3 .. 19, the last ten; sequence 1: rows 20 .. 59, the last 33
+        c, s = U.encode(k[first:first + n[b]], torch.int8)
+        p, o = pages.rows(b, n[b])
+        assert torch.equal(cache.k[p, :, o].cpu().double(), c) and torch.equal(cache.k_scale[p, :, o].cpu(), s)
+    kk, vv = (torch.full((50, 2, 64), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    cache.read(pages.table, ints([2, 12, 45]), k=kk, v=vv)
+    assert (kk[:2] == 7).all() and (kk[45:] == 7).all() and (vv[:2] == 7).all() and (vv[45:] == 7).all()
+    whole = cache.read(pages.table, U.offsets([10, 33]))
+    assert torch.equal(kk[2:45], whole[0]) and torch.equal(vv[2:45], whole[1])
+
+
 def test_bad_pages_are_reported_and_not_touched(cuda):
     """Page numbers outside the cache, and positions behind the table: an error status, no access, the rest right."""
     cache, pages = make(torch.int8, [40, 40], 16, 2, 64)
@@ -460,6 +479,26 @@ def test_paged_not_finite(cuda):
     cache.k[p[201], 1, o[201]] = float("nan")
     got = mb.attention_paged(q, cache, pages.table, ints(lengths))
     assert got[1, 4:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("width", [None, 300])
+def test_paged_not_finite_8_bit(cuda, dtype, width):
+    """A cached row that was NaN when it was written makes its group's output NaN, and nothing else; queries that are not
+    finite make theirs."""
+    cache, pages = filled(dtype, [70, 500], 16, 2, 128, 82, width=width)
+    q = rand((2, 6, 128), 83)
+    lens = ints([70, 500])
+    clean = mb.attention_paged(q, cache, pages.table, lens)
+    new = rand((2, 2, 128), 84)
+    new[1, 1, 7] = float("nan")
+    cache.write(new, rand((2, 2, 128), 85), pages.table, ints([0, 500]))
+    got = mb.attention_paged(q, cache, pages.table, lens)
+    assert torch.equal(got[0], clean[0]) and got[1, 3:].isnan().all() and torch.isfinite(got[1, :3]).all()
+    q[0, 2, 5], q[0, 4, 6] = float("inf"), float("nan")
+    got = mb.attention_paged(q, cache, pages.table, lens)
+    assert got[0, 2].isnan().all() and got[0, 4].isnan().all()
+    assert torch.equal(got[0, [0, 1, 3, 5]], clean[0, [0, 1, 3, 5]])
 
 
 def test_paged_offsets_past_32_bits(cuda):
