@@ -2,7 +2,7 @@
 // one f32 scale for each row of head_dim values) and read back.
 //
 // A group of head_dim / 16 threads owns a (token, head) row of k and the same row of v, two times 16 bytes
-// of bf16 a thread; the groups of a warp work on neighbouring rows and search for the sequence together,
+// of bf16 a thread; the groups of a warp work on neighbouring tokens and search for the sequence together,
 // while the rows are on their way. Bound by HBM, with little to spare for instructions: hence packed f32
 // arithmetic and no integer conversions or divisions (with them: 61 to 68 % of the issue slots, 55 us
 // where it is 41 for 11k rows of 8 x 128 written and 25k read, int8). More rows a thread or larger blocks
@@ -71,10 +71,13 @@ MB_DEV uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Token and head of a row.
-MB_DEV void split_row(int64_t row, int heads, int64_t& t, int& h) {
-  t = row < (1LL << 32) ? (int64_t)((uint32_t)row / (uint32_t)heads) : row / heads;
-  h = (int)(row - t * heads);
+// A block works on one head, its groups on neighbouring tokens: their rows and scales lie side by side in the cache, and
+// neighbouring blocks read the other heads of the same tokens. Token of the warp's first group:
+template <int SIDE>
+MB_DEV int64_t first_token(int heads, int& h) {
+  const uint32_t chunk = blockIdx.x / (uint32_t)heads;
+  h = (int)(blockIdx.x - chunk * heads);
+  return ((int64_t)chunk * (kThreads / 32) + (threadIdx.x >> 5)) * SIDE;
 }
 // On to the sequence that holds t, at or behind the present one.
 MB_DEV void advance(Span& s, const int32_t* cu, const int32_t* per_seq, int n, int64_t t) {
@@ -165,12 +168,9 @@ template <int CODES, int D>
 __global__ void __launch_bounds__(kThreads) k_kv_write(const WriteParams p) {
   constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
   const int lane = threadIdx.x % GROUP;
-  const int64_t row0 = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * SIDE;  // the warp's first
-  if (row0 >= p.n_tokens * p.c.heads) return;
-  int64_t t0, t;
-  int h0, h;
-  split_row(row0, p.c.heads, t0, h0);
-  split_row(row0 + (threadIdx.x & 31) / GROUP, p.c.heads, t, h);
+  int h;
+  const int64_t t0 = first_token<SIDE>(p.c.heads, h), t = t0 + (threadIdx.x & 31) / GROUP;
+  if (t0 >= p.n_tokens) return;
   const bool here = t < p.n_tokens;
   uint4 kx[kHalves], vx[kHalves];
 #pragma unroll
@@ -285,12 +285,9 @@ template <int CODES, int D>
 __global__ void __launch_bounds__(kThreads) k_kv_read(const ReadParams p) {
   constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
   const int lane = threadIdx.x % GROUP;
-  const int64_t row0 = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * SIDE;
-  if (row0 >= p.n_tokens * p.c.heads) return;
-  int64_t t0, t;
-  int h0, h;
-  split_row(row0, p.c.heads, t0, h0);
-  split_row(row0 + (threadIdx.x & 31) / GROUP, p.c.heads, t, h);
+  int h;
+  const int64_t t0 = first_token<SIDE>(p.c.heads, h), t = t0 + (threadIdx.x & 31) / GROUP;
+  if (t0 >= p.n_tokens) return;
   Span seq = seq_of(p.cu, nullptr, p.n_seqs, t0);
   if (t >= p.n_tokens) return;
   advance(seq, p.cu, nullptr, p.n_seqs, t);
@@ -308,8 +305,8 @@ __global__ void __launch_bounds__(kThreads) k_kv_read(const ReadParams p) {
 
 // Blocks for the rows of n_tokens tokens
 inline int64_t blocks_of(int64_t n_tokens, const mb_kv_cache* c) {
-  const int64_t per_block = kThreads / (c->head_dim / 16);
-  return (n_tokens * c->n_kv_heads + per_block - 1) / per_block;
+  const int64_t tokens = kThreads / (c->head_dim / 16);  // of a block
+  return (n_tokens + tokens - 1) / tokens * c->n_kv_heads;
 }
 
 // f(codes, head_dim) with both as types
