@@ -127,6 +127,18 @@ bool make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, const uint64_t (&dims)[4],
+                  const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swz) {
+  PFN_encodeTiled_t fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; i++) d[i] = dims[i], b[i] = box[i];
+  for (int i = 0; i < 3; i++) s[i] = stride_bytes[i];
+  return fn(map, dtype, 4, const_cast<void*>(base), d, s, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // ---------------------------------------------------------------- scratch
 static std::mutex g_scratch_mu;
 static void* g_scratch[64];

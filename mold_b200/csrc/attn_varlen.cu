@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if ((ok = wait(q_empty, (qn & 1) ^ 1))) {
           mbar_expect_tx(q_full, (uint32_t)(CH * G * TQ * 128));
           for (int c = 0; c < CH; c++)
-            tma_load_3d(sQ + c * S::kQHalf, &tq, q_full, c * 64, w.hk * G, w.q_start + w.tok0);
+            tma_load_4d(sQ + c * S::kQHalf, &tq, q_full, 0, w.hk * G, w.q_start + w.tok0, c);
           qn++;
         }
         // V of block j - 1 after K of block j: the scores need their K first
@@ -263,16 +263,14 @@ __global__ void __launch_bounds__(kThreads, 2)
             const int s = (kb + j) % kK;
             if (!(ok = wait(&k_empty[s], (((kb + j) / kK) & 1) ^ 1))) break;
             mbar_expect_tx(&k_full[s], S::kBlock);
-            for (int c = 0; c < CH; c++)
-              tma_load_3d(sK + s * S::kBlock + c * S::kHalf, &tk, &k_full[s], c * 64, w.hk, w.k_start + j * BKV);
+            tma_load_4d(sK + s * S::kBlock, &tk, &k_full[s], 0, w.hk, w.k_start + j * BKV, 0);
             nk++;
           }
           if (j > 0) {
             const int s = (kb + j - 1) % kV;
             if (!(ok = wait(&v_empty[s], (((kb + j - 1) / kV) & 1) ^ 1))) break;
             mbar_expect_tx(&v_full[s], S::kBlock);
-            for (int c = 0; c < CH; c++)
-              tma_load_3d(sV + s * S::kBlock + c * S::kHalf, &tv, &v_full[s], c * 64, w.hk, w.k_start + (j - 1) * BKV);
+            tma_load_4d(sV + s * S::kBlock, &tv, &v_full[s], 0, w.hk, w.k_start + (j - 1) * BKV, 0);
             nv++;
           }
         }
@@ -568,14 +566,17 @@ __global__ void __launch_bounds__(kThreads, 2)
 template <int D>
 cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, int64_t ldk, int H, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
-  const uint64_t head = D * 2, keys = p.total_k > 0 ? (uint64_t)p.total_k : 1;
-  // {channel, head, token}; a sequence's end inside a box reads the next sequence's rows, which the masks leave out
-  if (!make_tmap_3d(&tq, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)H, (uint64_t)p.total_q, head,
-                    (uint64_t)ldq * 2, 64, (uint32_t)p.G, (uint32_t)p.TQ, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_3d(&tk, k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)p.Hkv, keys, head,
-                    (uint64_t)ldk * 2, 64, 1, BKV, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      !make_tmap_3d(&tv, p.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, D, (uint64_t)p.Hkv, keys, head,
-                    (uint64_t)p.ldv * 2, 64, 1, BKV, CU_TENSOR_MAP_SWIZZLE_128B))
+  // {channel of an atom column, head, token, atom column}: the columns of a K or V block land behind each other in one
+  // copy (four copies of 32 rows in their place: 3 %); those of Q, whose boxes may be less than 128 rows, in one each. A
+  // sequence's end inside a box reads the next sequence's rows, which the masks leave out.
+  auto map = [&](CUtensorMap* m, const void* x, int64_t heads, int64_t rows, int64_t ld, int box_heads, int box_rows,
+                 int box_cols) {
+    return make_tmap_4d(m, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, {64, (uint64_t)heads, (uint64_t)(rows > 0 ? rows : 1), D / 64},
+                        {D * 2, (uint64_t)ld * 2, 128}, {64, (uint32_t)box_heads, (uint32_t)box_rows, (uint32_t)box_cols},
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  if (!map(&tq, q, H, p.total_q, ldq, p.G, p.TQ, 1) || !map(&tk, k, p.Hkv, p.total_k, ldk, 1, BKV, D / 64) ||
+      !map(&tv, p.v, p.Hkv, p.total_k, p.ldv, 1, BKV, D / 64))
     return cudaErrorInvalidValue;
   static int attr_done[64];
   int dev = 0;

@@ -52,6 +52,9 @@ bool make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
                   uint64_t d1, uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1,
                   uint32_t b2, CUtensorMapSwizzle swz);
 
+bool make_tmap_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, const uint64_t (&dims)[4],
+                  const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swz);
+
 // ---- per-device scratch (grown on demand; used by the f32-input path of mb_qlinear) ----
 void* device_scratch(size_t bytes);
 
