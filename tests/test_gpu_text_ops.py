@@ -92,6 +92,20 @@ def test_varlen_strided_views_and_rows_behind(cuda):
         mb.attention_varlen(q, k, v, U.offsets(ms), out=odd)
 
 
+@pytest.mark.parametrize("pad,start", [(0, 8), (8, 0), (8, 8), (0, 16), (0, 0)])
+def test_varlen_output_alignment(cuda, pad, start):
+    """Rows of out that begin at odd multiples of 16 bytes, all of them or every other one."""
+    T, H, Hkv, D = 77, 4, 2, 64
+    q, k, v = rand((T, H, D), 12), rand((T, Hkv, D), 13), rand((T, Hkv, D), 14)
+    flat = torch.full((T * (H * D + pad) + 32,), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = flat[start:].as_strided((T, H, D), (H * D + pad, D, 1))
+    want = mb.attention_varlen(q, k, v, ints([0, 30, T]))
+    mb.attention_varlen(q, k, v, ints([0, 30, T]), out=out)
+    assert torch.equal(out, want)
+    out.fill_(7.0)
+    assert (flat == 7).all()  # nothing beside the rows
+
+
 @pytest.mark.parametrize("H,Hkv,D", [(4, 4, 128), (16, 2, 64)])
 def test_varlen_what_is_masked_does_not_reach_a_row(cuda, H, Hkv, D):
     """NaN and infinities in keys and values of later positions, other sequences and unowned rows."""
