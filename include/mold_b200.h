@@ -421,10 +421,9 @@ enum { MB_KV_BF16 = 0, MB_KV_I8 = 1, MB_KV_E4M3 = 2 };
 /* A paged cache in caller-owned device memory. k, v: [n_pages, n_kv_heads, page_size, head_dim]
  * elements of `dtype`, 16-byte aligned; k_scale, v_scale: f32 [n_pages, n_kv_heads, page_size],
  * 16-byte aligned (NULL for MB_KV_BF16). page_size: a power of two, 16 to 256; fewer than 2^31
- * (page, head, position) rows. A sequence's
- * position p lies in page table[b][p / page_size] at offset p % page_size (table: device int32,
- * table_width pages of each sequence, rows ld_table apart); entries behind a sequence's last
- * page are not read. */
+ * (page, head, position) rows. A sequence's position p lies in page table[b][p / page_size] at
+ * offset p % page_size (table: device int32, table_width pages of each sequence, rows ld_table
+ * apart); entries behind a sequence's last page are not read. */
 typedef struct {
   void* k;
   void* v;
@@ -451,10 +450,11 @@ MB_API mb_status mb_attention_varlen(const void* q, int64_t ldq, const void* k, 
 /* K12. Append to the cache: sequence b's rows of k, v (bf16 [n_tokens, n_kv_heads, head_dim]) go
  * to its last positions, kv_lens[b] - m .. kv_lens[b] - 1 (kv_lens: device int32, the lengths
  * after the call). cu NULL: one row each (n_tokens == n_seqs). Rows that would come before
- * position 0 are passed over (kv_lens[b] <= 0: a sequence of a padded batch). MB_KV_BF16 keeps the values. The 8-bit types keep for each row of head_dim
- * values x the scale s = max|x| / T and the codes c nearest to x * (T / max|x|), ties to even
- * (scale, inverse and product rounded to f32; T = 127 or 448), standing for c * s. A row whose
- * largest magnitude is below 2^-100 is stored as zeros; one with a NaN or infinity reads back
+ * position 0 are passed over (kv_lens[b] <= 0: a sequence of a padded batch). MB_KV_BF16 keeps
+ * the values. The 8-bit types keep for each row of head_dim values x the scale s = max|x| / T and
+ * the codes c nearest to x * (T / max|x|), ties to even (scale, inverse and product rounded to
+ * f32; T = 127 or 448), standing for c * s. A row whose largest magnitude is below 2^-100 is
+ * stored as zeros; one with a NaN or infinity reads back
  * as NaN. A position is to be written once in a call: of two rows for one place (a page in two
  * table rows) either may stay, in part. */
 MB_API mb_status mb_kv_write(const mb_kv_cache* cache, const void* k, int64_t ldk, const void* v, int64_t ldv,
@@ -472,7 +472,8 @@ MB_API mb_status mb_kv_read(const mb_kv_cache* cache, const int32_t* cu, const i
  * (at most table_width * page_size): q bf16 [n_seqs, H, D], out bf16 likewise; a sequence without
  * positions gives 0. The cached lengths are split over the SMs and the parts joined in a fixed
  * order, so equal calls give equal bits. workspace: mb_attention_paged_workspace bytes of device
- * memory, 16-byte aligned, that no other call uses meanwhile (its contents need no setup). */
+ * memory, 16-byte aligned, that no other call uses meanwhile (its contents need no setup); the
+ * size depends on the current device, which has to be the call's. */
 MB_API mb_status mb_attention_paged_workspace(int n_seqs, int H, int H_kv, int D, size_t* bytes);
 MB_API mb_status mb_attention_paged(const void* q, int64_t ldq, const mb_kv_cache* cache, const int32_t* kv_lens,
                                     const int32_t* table, int64_t ld_table, int table_width, int n_seqs, int H,

@@ -445,8 +445,9 @@ class KVCache:
         got = self._workspaces.get((n_seqs, heads))
         if got is None:
             nbytes = ctypes.c_size_t(0)
-            check(lib().mb_attention_paged_workspace(n_seqs, heads, self.n_kv_heads, self.head_dim,
-                                                     ctypes.byref(nbytes)))
+            with torch.cuda.device(self.device_index):
+                check(lib().mb_attention_paged_workspace(n_seqs, heads, self.n_kv_heads, self.head_dim,
+                                                         ctypes.byref(nbytes)))
             got = self._workspaces[n_seqs, heads] = nbytes.value
         return got
 
