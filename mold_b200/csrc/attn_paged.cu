@@ -258,6 +258,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     *abort_flag = 0;
     fence_mbar_init();
   }
+  wait_before();
   auto length = [&](int b) -> int64_t {
     if (b >= p.n_seqs) return 0;
     const int64_t n = __ldg(p.lens + b);
@@ -757,12 +758,11 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
 }
 
 // Adds up the parts of each unit that several blocks hold, in the blocks' order; one block for each unit and query row.
-// Launched while k_attention_paged still runs (programmatic launch): it waits for that grid before it reads anything.
 constexpr int kJoinWarps = 4;
 template <int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const Params p) {
   __shared__ float4 s_acc[kJoinWarps][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_before();
   const int u = blockIdx.x, r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = u / p.units_per_seq, unit = u - b * p.units_per_seq;
   const int hk = unit / p.q_tiles, qt = unit - hk * p.q_tiles;
@@ -846,18 +846,8 @@ cudaError_t launch_attention(const Params& p, int64_t units, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     attr_done[dev & 63] = 1;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CLUSTER ? units * kCluster : num_sms() * S::BLOCKS));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = kCluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = CLUSTER ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, tk, tv, p);
+  return launch_close(kernel, dim3((unsigned)(CLUSTER ? units * kCluster : num_sms() * S::BLOCKS)), kThreads, S::kSmem, st,
+                      CLUSTER ? kCluster : 1, tk, tv, p);
 }
 
 template <int CODES, int D, bool WIDE>
@@ -872,16 +862,7 @@ cudaError_t launch(const Params& p, int64_t units, cudaStream_t st) {
   cudaError_t e = launch_attention<CODES, D, WIDE, false>(p, units, st);
   // a unit that fits a tile is never split
   if (e != cudaSuccess || keys <= kTileKeys) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)units, (unsigned)(p.G < kRows ? p.G : kRows));
-  cfg.blockDim = dim3(32 * kJoinWarps);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_join<D>, p);
+  return launch_close(k_join<D>, dim3((unsigned)units, (unsigned)(p.G < kRows ? p.G : kRows)), 32 * kJoinWarps, 0, st, 1, p);
 }
 
 template <int CODES, int D>

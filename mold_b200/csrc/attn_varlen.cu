@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
+  wait_before();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -604,8 +605,7 @@ cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, i
   }
   const int64_t blocks = (p.total_q / p.TQ + p.n_seqs) * p.Hkv;  // each sequence rounds up once
   if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  k_attention_varlen<D><<<(unsigned)blocks, kThreads, Smem<D>::kBytes, st>>>(tq, tk, tv, p);
-  return cudaGetLastError();
+  return launch_close(k_attention_varlen<D>, dim3((unsigned)blocks), kThreads, Smem<D>::kBytes, st, 1, tq, tk, tv, p);
 }
 
 }  // namespace varlen

@@ -86,6 +86,31 @@ MB_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
 }
 
 // ---------------------------------------------------------------- CTA pairs (clusters of 2)
+// ---------------------------------------------------------------- launches that follow each other closely
+// A kernel launched by launch_close may be set up while the one before it in its stream ends, and waits for that one with
+// wait_before() ahead of its first access to global memory. 1 to 1.5 us a launch (cache write and read, 40 sequences, e4m3:
+// 28.8 -> 25.3 us); letting the next one start before this one's blocks end gained nothing more.
+MB_DEV void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P>
+cudaError_t launch_close(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster,
+                         const P&... args) {
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 MB_DEV uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

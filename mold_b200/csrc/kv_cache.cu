@@ -167,6 +167,7 @@ MB_DEV void encode_row(const uint4 (&x)[kHalves], uint2 (&out)[kHalves], float& 
 
 template <int CODES, int D>
 __global__ void __launch_bounds__(kThreads) k_kv_write(const WriteParams p) {
+  wait_before();
   constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
   const int lane = threadIdx.x % GROUP;
   int h;
@@ -284,6 +285,7 @@ MB_DEV uint4 decode_row(const Held<CODES>& r, int j) {
 
 template <int CODES, int D>
 __global__ void __launch_bounds__(kThreads) k_kv_read(const ReadParams p) {
+  wait_before();
   constexpr int GROUP = D / 16, SIDE = 32 / GROUP;
   const int lane = threadIdx.x % GROUP;
   int h;
@@ -393,8 +395,8 @@ mb_status mb_kv_write(const mb_kv_cache* cache, const void* k, int64_t ldk, cons
   const kv::WriteParams p = {device_cache(cache), (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, ldk, ldv, n_tokens,
                              cu, kv_lens, table, ld_table, table_width, n_seqs, device_status_ptr()};
   MB_CUDA(kv::dispatch(cache, [&](auto codes, auto dim) {
-    kv::k_kv_write<decltype(codes)::value, decltype(dim)::value><<<(unsigned)blocks, kv::kThreads, 0, (cudaStream_t)stream>>>(p);
-    return cudaGetLastError();
+    return launch_close(kv::k_kv_write<decltype(codes)::value, decltype(dim)::value>, dim3((unsigned)blocks), kv::kThreads, 0,
+                        (cudaStream_t)stream, 1, p);
   }));
   return MB_OK;
 }
@@ -417,8 +419,8 @@ mb_status mb_kv_read(const mb_kv_cache* cache, const int32_t* cu, const int32_t*
   const kv::ReadParams p = {device_cache(cache), cu, table, ld_table, table_width, n_seqs, n_tokens,
                             (__nv_bfloat16*)k, (__nv_bfloat16*)v, ldk, ldv, device_status_ptr()};
   MB_CUDA(kv::dispatch(cache, [&](auto codes, auto dim) {
-    kv::k_kv_read<decltype(codes)::value, decltype(dim)::value><<<(unsigned)blocks, kv::kThreads, 0, (cudaStream_t)stream>>>(p);
-    return cudaGetLastError();
+    return launch_close(kv::k_kv_read<decltype(codes)::value, decltype(dim)::value>, dim3((unsigned)blocks), kv::kThreads, 0,
+                        (cudaStream_t)stream, 1, p);
   }));
   return MB_OK;
 }

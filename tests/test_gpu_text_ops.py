@@ -612,3 +612,65 @@ def test_small_workspace_refused(cuda):
                                      pages.table.data_ptr(), pages.table.shape[1], pages.table.shape[1], 1, 2, 0.0,
                                      q.data_ptr(), 128, ws.data_ptr(), 64, None)
     assert rc == _lib.MB_ERR_INVALID and b"workspace" in mb.lib().mb_last_error()
+
+
+@pytest.mark.parametrize("how", ["stream", "other_stream", "graph", "graph_copy", "graph_other_stream"])
+def test_calls_wait_for_what_came_before(cuda, how):
+    """Inputs that a slow kernel, a copy or another stream has only just made, eagerly and in captured graphs; and each call
+    right behind the one whose results it takes."""
+    H, Hkv, D, lengths = 6, 2, 128, [70, 33]
+    cache, pages = make(torch.int8, lengths, 16, Hkv, D)
+    lens, cu, T = ints(lengths), U.offsets(lengths), sum(lengths)
+    src = [[rand(s, 150 + 10 * i + j) for j, s in enumerate(((T, H, D), (T, Hkv, D), (T, Hkv, D)))] for i in range(2)]
+    now = [torch.empty_like(x) for x in src[0]]
+    held = [torch.empty_like(x) for x in src[0]]
+    kk, vv = torch.empty_like(src[0][1]), torch.empty_like(src[0][2])
+    out, last = torch.empty_like(src[0][0]), torch.empty((2, H, D), device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+
+    def make_inputs():
+        torch.cuda._sleep(400000)  # clocks
+        for x, y in zip(now, held):
+            if how == "graph_copy":
+                x.copy_(y)
+            else:
+                torch.add(y, 0.0, out=x)
+
+    def calls():
+        cache.write(now[1], now[2], pages.table, lens, cu=cu)
+        cache.read(pages.table, cu, k=kk, v=vv)
+        mb.attention_varlen(now[0], kk, vv, cu, out=out)
+        mb.attention_paged(out[cu[1:].long() - 1] if graph is None else out[:2], cache, pages.table, lens, out=last)
+
+    def run():
+        if "other" in how:
+            here = torch.cuda.current_stream()
+            side.wait_stream(here)
+            with torch.cuda.stream(side):
+                make_inputs()
+            here.wait_stream(side)
+        else:
+            make_inputs()
+        calls()
+
+    graph = torch.cuda.CUDAGraph() if "graph" in how else None
+    refs = []
+    for inputs in src:
+        for x, y in zip(now, inputs):
+            x.copy_(y)
+        torch.cuda.synchronize()
+        calls()
+        torch.cuda.synchronize()
+        refs.append([x.clone() for x in (kk, vv, out, last)])
+    if graph is not None:
+        with torch.cuda.graph(graph):
+            run()
+    for i in (0, 1, 1, 0, 1):
+        for x, y in zip(held, src[i]):
+            x.copy_(y)
+        for x in (kk, vv, out, last):
+            x.fill_(float("nan"))
+        run() if graph is None else graph.replay()
+        got = [x.clone() for x in (kk, vv, out, last)]
+        assert all(torch.equal(x, y) for x, y in zip(got, refs[i]))
+    assert mb.device_status() == 0
