@@ -31,7 +31,7 @@
 //   * 2^11, relative to 2^-11 down to 2^-25 of the largest and to 2^-36 of it below.
 // Converting codes to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
 //
-// Bound by HBM: 64 sequences of 64 to 4096 keys, 32 / 8 heads of 128, bf16: 51.5 us, 5.1 TB/s, and 2 of 100001 to 131072, int8:
+// Bound by HBM: 64 sequences of 64 to 4096 keys, 32 / 8 heads of 128, bf16: 50.9 us, 5.2 TB/s, and 2 of 100001 to 131072, int8:
 // 98 us, 5.3 TB/s; a plain sum over as many bytes takes 51.0 and 94.8 us. 160 of 256 to 8192, 64 / 8 heads, e4m3: 161 us, 5.0
 // TB/s, where the conversion of codes shows (144 us without the products).
 #include <math.h>

@@ -5,9 +5,9 @@
 // of bf16 a thread; the groups of a warp work on neighbouring tokens and search for the sequence together,
 // while the rows are on their way. Bound by HBM, with little to spare for instructions: hence packed f32
 // arithmetic and no integer conversions or divisions (with them: 61 to 68 % of the issue slots, 55 us
-// where it is 39.7, 5.4 TB/s, for 11k rows of 8 x 128 written and 25k read, int8). More rows a thread or larger
+// where it is 38.8, 5.6 TB/s, for 11k rows of 8 x 128 written and 25k read, int8). More rows a thread or larger
 // blocks lose (2 rows: 41.2, 4: 48 us; a generation step 6.1 and 9.6 against 4.8 us), and so do accesses of 32
-// bytes (40.4).
+// bytes (40.4 against 39.9).
 #include <string>
 
 #include "common.cuh"

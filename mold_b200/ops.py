@@ -483,14 +483,16 @@ class KVCache:
         if (k is None) != (v is None):
             raise ValueError("give both k and v or neither")
         if k is None:
-            n_tokens = int(cu[-1]) if n_tokens is None else int(n_tokens)
-            shape = (n_tokens, self.n_kv_heads, self.head_dim)
-            k = torch.empty(*shape, dtype=torch.bfloat16, device=self.k.device)
+            rows = int(cu[-1]) if n_tokens is None else int(n_tokens)
+            k = torch.empty((rows, self.n_kv_heads, self.head_dim), dtype=torch.bfloat16, device=self.k.device)
             v = torch.empty_like(k)
-        k, k_ptr, ldk, rows = self._rows(k, "k", copy=False)
-        v, v_ptr, ldv, v_rows = self._rows(v, "v", copy=False)
-        if rows != v_rows or (n_tokens is not None and n_tokens != rows):
-            raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} and n_tokens {n_tokens} do not fit")
+            k_ptr, v_ptr, ldk = k.data_ptr(), v.data_ptr(), self.n_kv_heads * self.head_dim
+            ldv = ldk
+        else:
+            k, k_ptr, ldk, rows = self._rows(k, "k", copy=False)
+            v, v_ptr, ldv, v_rows = self._rows(v, "v", copy=False)
+            if rows != v_rows or (n_tokens is not None and n_tokens != rows):
+                raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} and n_tokens {n_tokens} do not fit")
         table, t_ptr, ldt, width = _table(table, n)
         _launch(dev, lib().mb_kv_read, self._ref, cu_ptr, t_ptr, ldt, width, n, rows, k_ptr, ldk, v_ptr, ldv)
         return k, v
