@@ -71,6 +71,7 @@ struct Params {
   int64_t ld_table;
   int table_width, n_seqs;
   int H, G, q_tiles, units_per_seq;
+  int box;  // 16-key groups of a tile that one copy brings: 1, 2 or 4, as a page holds them
   float scale_log2;
   __nv_bfloat16* out;
   int64_t ldo;
@@ -97,6 +98,13 @@ MB_DEV void mma16816_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+MB_DEV void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Arrives once the thread's copies so far are there.
+MB_DEV void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // A float of another block of the cluster, at the place of p in this one.
 MB_DEV float ld_cluster(const float* p, int rank) {
@@ -250,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
   const int U = p.units_per_seq;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], CODES == MB_KV_BF16 ? 1 : 33);  // and 32 lanes' copies of scales
       mbar_init(&empty[i], kWarps);
     }
     for (int i = 0; i < S::QSLOTS; i++) mbar_init(&q_empty[i], kWarps);
@@ -384,23 +392,30 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
           d.slot = whole ? -1 : 2 * c + (kt0 == 0 ? 1 : 0);
           d.end = d.last && end;
           desc[s] = d;
-          mbar_expect_tx(&full[s], __popc(groups) * 2u * (16 * S::ROWB + S::SCALEB / kWarps) + q_bytes);
+          const unsigned firsts = p.box == 4 ? 1 : p.box == 2 ? 5 : 15;  // groups that begin a box
+          mbar_expect_tx(&full[s], __popc(groups & firsts) * p.box * 2u * 16 * S::ROWB + q_bytes);
         }
         __syncwarp();
-        // lane 8 i + j: copy j of group i (planes of K, planes of V, scales of K, of V)
+        // lane 8 i + j: copy j of the box that begins with group i (planes of K, planes of V); keys of a
+        // page behind the sequence's end come along
         const int gi = lane >> 3, j = lane & 7;
         const int64_t grow = __shfl_sync(0xffffffffu, row32, ahead + gi);
-        if (grow >= 0) {
+        if (grow >= 0 && (gi & (p.box - 1)) == 0) {
           if (j < 2 * S::PLANES) {
             const int plane = j % S::PLANES;
             const bool is_v = j >= S::PLANES;
             uint8_t* dst = st + (is_v ? S::KVB : 0) + plane * S::PLANEB + gi * S::GROUPB;
             // rows shorter than a line lie two to a line of the map
             tma_load_2d(dst, is_v ? &tv : &tk, &full[s], plane * 128, (int)(grow * S::LINEB / 128));
-          } else if (CODES != MB_KV_BF16 && j >= 4 && j < 6) {
-            bulk_load(st + 2 * S::KVB + (j == 5 ? S::SCALEB : 0) + gi * 64, (j == 5 ? p.c.v_scale : p.c.k_scale) + grow, 64,
-                      &full[s]);
           }
+        }
+        if (CODES != MB_KV_BF16) {
+          // scales: 16 bytes a lane of K (0-15) or V. Bulk copies of 64 bytes took as long to issue as those of the rows.
+          const int i = lane & 15;
+          const int64_t from = __shfl_sync(0xffffffffu, row32, ahead + (i >> 2));
+          if (from >= 0)
+            cp_async16(st + 2 * S::KVB + (lane >> 4) * S::SCALEB + i * 16, (lane >> 4 ? p.c.v_scale : p.c.k_scale) + from + (i & 3) * 4);
+          cp_async_arrive(&full[s]);
         }
         if (lane == 31 && q_bytes)
           bulk_load(s_q + qs * S::QB, p.q + (int64_t)b * p.ldq + (int64_t)(hk * p.G + qt * kRows) * D, q_bytes, &full[s]);
@@ -835,7 +850,7 @@ cudaError_t launch_attention(const Params& p, int64_t units, cudaStream_t st) {
   const uint64_t rows = ((uint64_t)p.c.n_pages * p.c.heads << p.c.page_log2) * S::ROWB / inner;
   for (int i = 0; i < 2; i++)
     if (!make_tmap_2d(i ? &tv : &tk, i ? p.c.v : p.c.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, inner, rows, inner, 128,
-                      S::GROUPB / 128, CU_TENSOR_MAP_SWIZZLE_128B))
+                      S::GROUPB / 128 * p.box, CU_TENSOR_MAP_SWIZZLE_128B))
       return cudaErrorInvalidValue;
   auto kernel = k_attention_paged<CODES, D, WIDE, CLUSTER>;
   static int attr_done[64];
@@ -926,6 +941,7 @@ mb_status mb_attention_paged(const void* q, int64_t ldq, const mb_kv_cache* cach
   p.G = H / cache->n_kv_heads;
   p.q_tiles = (p.G + paged::kRows - 1) / paged::kRows;
   p.units_per_seq = cache->n_kv_heads * p.q_tiles;
+  p.box = cache->dtype == MB_KV_BF16 ? 1 : cache->page_size >= paged::kTileKeys ? 4 : cache->page_size / 16;
   p.scale_log2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)D)) * 1.4426950408889634);
   p.out = (__nv_bfloat16*)out;
   p.ldo = ldo;
