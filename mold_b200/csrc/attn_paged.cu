@@ -8,8 +8,8 @@
 // unit that it does not hold whole goes to the workspace as (max, sum, unnormalised output); k_join adds
 // a unit's parts in the order of the blocks.
 //
-// One warp of a block walks the run and keeps a ring of tiles in flight: page numbers, one TMA box of 16
-// keys x 128 bytes after the other (keys, values; 128-byte swizzle), scales and the unit's queries, all
+// One warp of a block walks the run and keeps a ring of tiles in flight: page numbers, one TMA box of 16 to
+// 64 keys x 128 bytes after the other (keys, values; 128-byte swizzle), scales and the unit's queries, all
 // landing on the stage's mbarrier. It runs ahead over the borders of units, so a batch of short
 // sequences keeps memory as busy as a long one. Four warps take 16 keys of a tile each: q k^T and p v as
 // warp products (query heads as rows; at one token a row there is too little arithmetic for more). Which
@@ -31,9 +31,9 @@
 //   * 2^11, relative to 2^-11 down to 2^-25 of the largest and to 2^-36 of it below.
 // Converting codes to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
 //
-// Bound by HBM: 64 sequences of 64 to 4096 keys, 32 / 8 heads of 128, bf16: 50.9 us, 5.2 TB/s, and 2 of 100001 to 131072, int8:
-// 98 us, 5.3 TB/s; a plain sum over as many bytes takes 51.0 and 94.8 us. 160 of 256 to 8192, 64 / 8 heads, e4m3: 161 us, 5.0
-// TB/s, where the conversion of codes shows (144 us without the products).
+// Bound by HBM: 64 sequences of 64 to 4096 keys, 32 / 8 heads of 128, bf16: 50.9 us, 5.2 TB/s; 2 of 100001 to 131072, int8:
+// 87 us, 5.9 TB/s; 160 of 256 to 8192, 64 / 8 heads, e4m3: 146 us, 5.5 TB/s. A plain sum over as many bytes takes 51.0, 94.8 and
+// 139 us. More than 8 heads a key head over 8-bit caches are bound by the products' latency (16 heads of 128: 3.6 to 4.1 TB/s).
 #include <math.h>
 
 #include <string>
@@ -48,7 +48,7 @@ namespace paged {
 constexpr int kWarps = 4;                   // that compute; one more loads
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kRows = 16;                   // query rows of a unit
-constexpr int kMaxBlocksPerSm = 3;
+constexpr int kMaxBlocksPerSm = 4;
 constexpr int kTileKeys = 16 * kWarps;
 constexpr int kCluster = 8;
 constexpr float kSlack = 4.f;               // log2 of how far a weight may pass 1
@@ -185,7 +185,10 @@ struct Shape {
   static constexpr int MERGE_PITCH = NR * 16 + 4;   // floats; rows 2t begin 8 banks apart
   static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
   static constexpr int UNIT_COST = CODES == MB_KV_BF16 ? 3 : 8;
-  static constexpr int BLOCKS = CODES == MB_KV_BF16 || WIDE ? 2 : 3;  // on an SM
+  // Blocks on an SM, as many as registers allow where there is little arithmetic in flight: 64 sequences of 8000, 8 key heads of
+  // 64, int8: 114 us with 3, 108 with 4 (4 heads a key head); 168 with 2, 157 with 3 (16). Heads of 128 spill instead (16:
+  // 148 us with 2, 193 with 3).
+  static constexpr int BLOCKS = CODES == MB_KV_BF16 ? 2 : D == 64 ? (WIDE ? 3 : 4) : (WIDE ? 2 : 3);
   static constexpr int kBudget = (228 / BLOCKS - 2) * 1024;  // of a block: 1 KB is the system's, 1 KB for alignment
   static constexpr int kFixed = QSLOTS * QB + MERGEB + 2 * kWarps * kRows * 4 + 1024;  // and barriers, descriptors
   static constexpr int STAGES = (kBudget - kFixed) / STAGEB < 8 ? (kBudget - kFixed) / STAGEB : 8;
@@ -414,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
           const int i = lane & 15;
           const int64_t from = __shfl_sync(0xffffffffu, row32, ahead + (i >> 2));
           if (from >= 0)
-            cp_async16(st + 2 * S::KVB + (lane >> 4) * S::SCALEB + i * 16, (lane >> 4 ? p.c.v_scale : p.c.k_scale) + from + (i & 3) * 4);
+            cp_async16(st + 2 * S::KVB + (lane >> 4) * S::SCALEB + i * 16,
+                       (lane >> 4 ? p.c.v_scale : p.c.k_scale) + from + (i & 3) * 4);
           cp_async_arrive(&full[s]);
         }
         if (lane == 31 && q_bytes)
@@ -941,6 +945,8 @@ mb_status mb_attention_paged(const void* q, int64_t ldq, const mb_kv_cache* cach
   p.G = H / cache->n_kv_heads;
   p.q_tiles = (p.G + paged::kRows - 1) / paged::kRows;
   p.units_per_seq = cache->n_kv_heads * p.q_tiles;
+  // 8-bit: with 16 keys a copy the loading warp was behind (64 sequences of 8000, heads of 64, 162 us against 116). bf16 has
+  // twice the bytes in a copy, and would read keys behind the end for nothing (64 sequences of 64 to 4096: 50.7 against 52.1).
   p.box = cache->dtype == MB_KV_BF16 ? 1 : cache->page_size >= paged::kTileKeys ? 4 : cache->page_size / 16;
   p.scale_log2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)D)) * 1.4426950408889634);
   p.out = (__nv_bfloat16*)out;
