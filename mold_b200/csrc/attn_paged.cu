@@ -56,7 +56,8 @@ constexpr float kWeightOne = 2048.f;        // f16 form of a weight of 1 with th
 
 // Cost of a tile. A unit costs Shape::UNIT_COST besides its tiles (queries, joining the warps, output), more beside the
 // smaller tiles of an 8-bit cache. Without it blocks with many short units end last: 64 sequences up to 4096, bf16, cost
-// 0 / 3 / 6 / 12: 55.4 / 51.3 / 51.6 / 52.8 us; 160 up to 8192, e4m3, 0 / 3 / 8 / 12: 177 / 169 / 162 / 163 us.
+// 0 / 3 / 6 / 12: 55.4 / 51.3 / 51.6 / 52.8 us; 160 up to 8192, e4m3, 8 / 12 / 16: 146 / 143 / 143 us; 512 of 30 to 600, int8,
+// 8 / 16 / 24: 111 / 104 / 105 us; others lose past 16.
 constexpr int kTileCost = 4;
 
 struct Part {  // of a unit's work: its first block and how many blocks hold a piece (1: none is joined)
@@ -184,7 +185,7 @@ struct Shape {
   static constexpr int NR = WIDE ? 2 : 4;           // 16-channel output tiles that are merged at a time
   static constexpr int MERGE_PITCH = NR * 16 + 4;   // floats; rows 2t begin 8 banks apart
   static constexpr int MERGEB = kWarps * ROWS * MERGE_PITCH * 4;
-  static constexpr int UNIT_COST = CODES == MB_KV_BF16 ? 3 : 8;
+  static constexpr int UNIT_COST = CODES == MB_KV_BF16 ? 3 : 12;
   // Blocks on an SM, as many as registers allow where there is little arithmetic in flight: 64 sequences of 8000, 8 key heads of
   // 64, int8: 114 us with 3, 108 with 4 (4 heads a key head); 168 with 2, 157 with 3 (16). Heads of 128 spill instead (16:
   // 148 us with 2, 193 with 3).
