@@ -423,7 +423,9 @@ enum { MB_KV_BF16 = 0, MB_KV_I8 = 1, MB_KV_E4M3 = 2 };
  * 16-byte aligned (NULL for MB_KV_BF16). page_size: a power of two, 16 to 256; fewer than 2^31
  * (page, head, position) rows. A sequence's position p lies in page table[b][p / page_size] at
  * offset p % page_size (table: device int32, table_width pages of each sequence, rows ld_table
- * apart); entries behind a sequence's last page are not read. */
+ * apart); entries behind a sequence's last page are not read. The scales may come from another
+ * writer: any finite numbers, of either sign (what is not finite makes what sees it NaN or
+ * infinite). */
 typedef struct {
   void* k;
   void* v;

@@ -27,8 +27,9 @@
 //   e4m3 scores: codes to f16, which holds every code, with the query row times a power of two in f16 (off
 //   by at most 2^-25 of the row's largest magnitude). The 8-bit float product is no help here: it measured
 //   as many instructions as the conversion.
-//   Values become f16, and the weights are rounded to f16 as p * (value scale / largest value scale so far)
-//   * 2^11, relative to 2^-11 down to 2^-25 of the largest and to 2^-36 of it below.
+//   Values become f16, and the weights are rounded to f16 as p * (value scale / largest magnitude of a value
+//   scale so far) * 2^11, relative to 2^-11 down to 2^-25 of the largest and to 2^-36 of it below. Scales may
+//   be any finite numbers, of either sign.
 // Converting codes to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
 //
 // Bound by HBM: 64 sequences of 64 to 4096 keys, 32 / 8 heads of 128, bf16: 50.9 us, 5.2 TB/s; 2 of 100001 to 131072, int8:
@@ -53,6 +54,8 @@ constexpr int kTileKeys = 16 * kWarps;
 constexpr int kCluster = 8;
 constexpr float kSlack = 4.f;               // log2 of how far a weight may pass 1
 constexpr float kWeightOne = 2048.f;        // f16 form of a weight of 1 with the largest value scale: 2^15 at most
+constexpr float kLeastScale = 2.407412430484045e-35f;  // 2^-115: smaller value scales count as this, so that kWeightOne over
+                                                       // the largest is finite (2^126 at most)
 
 // Cost of a tile. A unit costs Shape::UNIT_COST besides its tiles (queries, joining the warps, output), more beside the
 // smaller tiles of an 8-bit cache. Without it blocks with many short units end last: 64 sequences up to 4096, bf16, cost
@@ -449,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     float q_size[RR][2];
     // o: channels 16 i + g (0, 1) and + 8 (2, 3) of rows 8 r + 2t and + 1; m, l: of these rows
     float o[RR][D / 16][4], m[RR][2], l[RR][2];
-    float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest value scale so far, and kWeightOne over it
+    float v_ref = 0.f, v_inv = 0.f;  // 8-bit: largest magnitude of a value scale so far, and kWeightOne over it
     uint32_t merges = 0;
     for (int it = 0;; it++) {
       const int s = it % STAGES;
@@ -577,8 +580,8 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
           vs_a = in_a ? scale[kTileKeys + key_a] : 0.f, vs_b = in_b ? scale[kTileKeys + key_b] : 0.f;
         }
         // The reference points move (and the output with them) only when a score passes its row's by more than 2^kSlack,
-        // or a value scale the largest so far.
-        bool move = !B16 && fmaxf(vs_a, vs_b) > v_ref;
+        // or a value scale's magnitude the largest so far.
+        bool move = !B16 && fmaxf(fabsf(vs_a), fabsf(vs_b)) > v_ref;
 #pragma unroll
         for (int r = 0; r < RR; r++)
 #pragma unroll
@@ -594,10 +597,11 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
         if (__any_sync(0xffffffffu, move)) {
           float shrink = 1.f;
           if (!B16) {
-            float vm = fmaxf(vs_a, vs_b);
+            float vm = fmaxf(fabsf(vs_a), fabsf(vs_b));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, x));
             if (vm > v_ref) {  // the same in all lanes
+              vm = fmaxf(vm, kLeastScale);
               shrink = v_ref / vm;
               v_ref = vm;
               v_inv = kWeightOne / vm;

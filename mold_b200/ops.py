@@ -413,7 +413,8 @@ class KVCache:
 
     @classmethod
     def from_tensors(cls, k, v, k_scale=None, v_scale=None):
-        """A cache over tensors that the caller has; they are used in place."""
+        """A cache over tensors that the caller has; they are used in place. Scales that this library did not write may be
+        any finite numbers."""
         self = cls.__new__(cls)
         self._hold(k, v, k_scale, v_scale)
         return self
