@@ -1,5 +1,6 @@
-"""One-token attention over 8-bit caches whose scales range widely: of either sign and next to the smallest numbers.
-Against a 64-bit restatement over the numbers that the cache holds."""
+"""One-token attention over 8-bit caches where scales and scores range widely: value scales over many powers of two, of
+either sign and next to the smallest numbers, growing scores, queries with an outlying channel. Against a 64-bit
+restatement over the numbers that the cache holds."""
 import math
 
 import pytest
@@ -71,6 +72,77 @@ def tables(pages):
     wide = torch.full((pages.table.shape[0], 400), -1, dtype=torch.int32, device="cuda")
     wide[:, :pages.table.shape[1]] = pages.table
     return pages.table, wide
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+@pytest.mark.parametrize("order", ["ascending", "descending", "zeros_first", "shuffled"])
+def test_value_scales_over_many_powers(cuda, dtype, H, Hkv, D, order):
+    """Rows of V from 2^-20 to 2^10 along the length, on growing keys: the reference of the value scales moves by orders of
+    magnitude, and differs between warps, blocks and parts."""
+    lengths = [1000, 77, 0, 2500]
+    pages = U.Pages(lengths, 16, seed=3)
+    cache = mb.KVCache(pages.n_pages, 16, Hkv, D, dtype)
+    T = sum(lengths)
+    k, v = rand((T, Hkv, D), 1), rand((T, Hkv, D), 2)
+    at = 0
+    for n in lengths:
+        if n:
+            e = torch.linspace(-20, 10, n, device="cuda")
+            if order == "descending":
+                e = e.flip(0)
+            elif order == "shuffled":
+                e = e[torch.randperm(n, generator=torch.Generator().manual_seed(n)).cuda()]
+            f = torch.exp2(e)
+            if order == "zeros_first":
+                f[:n // 3] = 0
+            v[at:at + n] *= f[:, None, None].bfloat16()
+            k[at:at + n] *= torch.linspace(0.1, 3.0, n, device="cuda")[:, None, None].bfloat16()
+        at += n
+    cache.write(k, v, pages.table, ints(lengths), cu=U.offsets(lengths))
+    q = rand((len(lengths), H, D), 4)
+    for table in tables(pages):
+        for scale in (None, 2.0 ** -9):
+            out = mb.attention_paged(q, cache, table, ints(lengths), scale=scale)
+            check(q, cache, pages, lengths, out, scale)
+    assert mb.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16] + TYPES)
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+def test_growing_scores(cuda, dtype, H, Hkv, D):
+    """Scores that keep growing along the length move the reference point again and again."""
+    lengths = [1500, 300]
+    pages = U.Pages(lengths, 32, seed=5)
+    cache = mb.KVCache(pages.n_pages, 32, Hkv, D, dtype)
+    k, v = rand((1800, Hkv, D), 11), rand((1800, Hkv, D), 12)
+    k *= torch.cat([torch.linspace(0.2, 8.0, n, device="cuda") for n in lengths])[:, None, None].bfloat16()
+    cache.write(k, v, pages.table, ints(lengths), cu=U.offsets(lengths))
+    q = rand((2, H, D), 13, 1.5)
+    for table in tables(pages):
+        out = mb.attention_paged(q, cache, table, ints(lengths))
+        if dtype != torch.bfloat16:
+            check(q, cache, pages, lengths, out)
+            continue
+        for b, n in enumerate(lengths):
+            kk, vv = U.cached64(cache, pages, b, n)
+            keep = torch.ones((1, n), dtype=torch.bool, device="cuda")
+            close(out[b:b + 1], *U.attention64(q[b:b + 1], kk, vv, keep))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,D", SHAPES)
+def test_queries_with_an_outlying_channel(cuda, dtype, H, Hkv, D):
+    """One channel of q far above the others, where the keys are small: the others' scores decide."""
+    lengths = [200]
+    pages = U.Pages(lengths, 64, seed=6)
+    cache = mb.KVCache(pages.n_pages, 64, Hkv, D, dtype)
+    k, v = rand((200, Hkv, D), 21), rand((200, Hkv, D), 22)
+    k[:, :, 3] = 0
+    cache.write(k, v, pages.table, ints(lengths), cu=U.offsets(lengths))
+    q = rand((1, H, D), 23)
+    q[:, :, 3] = 100.0
+    check(q, cache, pages, lengths, mb.attention_paged(q, cache, pages.table, ints(lengths)))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
