@@ -222,11 +222,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     *abort_flag = 0;
     fence_mbar_init();
   }
+  wait_before();  // ahead of the allocation: a block of the kernel before this one may need these columns to end
   if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
-  wait_before();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -85,11 +85,12 @@ MB_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
                : "memory");
 }
 
-// ---------------------------------------------------------------- CTA pairs (clusters of 2)
 // ---------------------------------------------------------------- launches that follow each other closely
 // A kernel launched by launch_close may be set up while the one before it in its stream ends, and waits for that one with
 // wait_before() ahead of its first access to global memory. 1 to 1.5 us a launch (cache write and read, 40 sequences, e4m3:
-// 28.8 -> 25.3 us); letting the next one start before this one's blocks end gained nothing more.
+// 28.8 -> 25.3 us); letting the next one start before this one's blocks end gained nothing more. The one before may be any
+// kernel of the stream, and may let this one's blocks in while blocks of its own still run: so nothing that those could wait
+// for (tensor memory above all) is held across the wait.
 MB_DEV void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <class... P>
@@ -111,6 +112,7 @@ cudaError_t launch_close(void (*kernel)(P...), dim3 grid, int threads, size_t sm
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// ---------------------------------------------------------------- CTA pairs (clusters of 2)
 MB_DEV uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
