@@ -82,6 +82,7 @@ struct Params {
   Part* parts;       // [units]
   float *part_ml;    // [2 * blocks][2][kRows]
   float *part_o;     // [2 * blocks][kRows][D]
+  int blocks;        // that the workspace has room for
   int* status;
 };
 
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     for (int i = 0; i < S::QSLOTS; i++) mbar_init(&q_empty[i], kWarps);
     mbar_init(merge_bar, kWarps);
     *abort_flag = 0;
+    *s_seq = -1;
     fence_mbar_init();
   }
   wait_before();
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     if (c >= n_blocks) return;
     x0 = run_start(total, c, n_blocks), x1 = run_start(total, c + 1, n_blocks);
     int64_t before = 0;
-    for (int base = 0;; base += kThreads) {
+    for (int base = 0; base < p.n_seqs; base += kThreads) {
       if (p.n_seqs > kThreads) incl = scan(base, all); else all = total;
       const int64_t own = S::unit_cost(tiles_of(length(base + (int)threadIdx.x))) * U;
       const int64_t end = before + incl;
@@ -339,9 +341,11 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
     __syncthreads();
     // the first unit of the run, and whether any tile begins in it
     b = *s_seq;
+    if (b < 0) return;  // here and below: lengths that changed under the call
     len = length(b), nt = tiles_of(len), at = *s_at;
-    if (nt == 0) return;  // lengths that changed under the call
+    if (nt == 0) return;
     unit = (int)((x0 - at) / S::unit_cost(nt));
+    if (unit >= U) return;
     at += unit * S::unit_cost(nt);
     if (S::tiles_before(at, nt, x0) >= S::tiles_before(at, nt, x1) &&
         (at + S::unit_cost(nt) >= total || at + S::unit_cost(nt) + S::UNIT_COST >= x1))
@@ -794,6 +798,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const Params p) {
   const int len = __ldg(p.lens + b);
   const Part part = p.parts[u];
   if (len <= 0 || part.pieces <= 1) return;
+  // left by another call where this one gave up a wait, or lengths changed under it
+  if (part.first < 0 || part.pieces > p.blocks - part.first) return;
   auto slot = [&](int i) { return (int64_t)2 * (part.first + i) + (i == 0 ? 1 : 0); };
   // every warp the statistics of all parts, 32 at a time
   float top = -INFINITY;
@@ -959,6 +965,7 @@ mb_status mb_attention_paged(const void* q, int64_t ldq, const mb_kv_cache* cach
   p.parts = (paged::Part*)workspace;
   p.part_ml = (float*)((char*)workspace + a.ml);
   p.part_o = (float*)((char*)workspace + a.o);
+  p.blocks = (int)a.blocks;
   p.status = device_status_ptr();
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;

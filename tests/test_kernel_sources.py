@@ -1,6 +1,8 @@
-"""What kernels that are launched close behind others (launch_close) may do before they wait for those, checked on the
-sources: such a block may be resident while the kernel before it still runs, so it holds no tensor memory that one of
-that kernel's blocks could be waiting for, and no thread ends, or reads what that kernel writes, ahead of its wait."""
+"""What the kernels promise and no test on a GPU may provoke, checked on the sources: what kernels that are launched close
+behind others (launch_close) do before they wait for those, and what the paged attention does with indices that a call which
+gave up has left. A block launched close may be resident while the kernel before it still runs, so it holds no tensor memory
+that one of that kernel's blocks could be waiting for, and no thread ends, or reads what that kernel writes, ahead of its
+wait."""
 import os
 import re
 
@@ -49,3 +51,26 @@ def test_nothing_before_the_wait(what):
     for f, name, body in close_kernels():
         before = body[:body.index("wait_before()")]
         assert what not in before, f"{f}: {name} has {what} ahead of wait_before()"
+
+
+def body(name):
+    return next(k[2] for k in kernels() if k[1] == name)
+
+
+def test_join_checks_the_parts_that_it_finds():
+    """A call that gave up a wait, or whose lengths changed under it, leaves parts unwritten: the join takes nothing from the
+    workspace as an index that it has not checked, and ends before its first access if it does not fit."""
+    b = body("k_join")
+    check = b.index("p.blocks - part.first")
+    assert "part.first < 0" in b[:check + 40] and check < b.index("p.part_ml[") and check < b.index("p.part_o +")
+
+
+def test_paged_search_ends_and_checks_what_it_found():
+    """Lengths that change while a block searches its first unit may leave it without one: the search ends with the last
+    sequence, and neither an index that was never written nor a unit behind the sequence's last is used."""
+    b = body("k_attention_paged")
+    search = b[b.index("int64_t before = 0"):b.index("b = *s_seq")]
+    assert "for (int base = 0; base < p.n_seqs; base += kThreads)" in search
+    assert "*s_seq = -1" in b[:b.index("wait_before()")]
+    after = b[b.index("b = *s_seq"):b.index("S::tiles_before(at, nt, x0) >=")]
+    assert after.index("if (b < 0) return") < after.index("length(b)") and "if (unit >= U) return" in after
