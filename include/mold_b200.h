@@ -442,8 +442,9 @@ typedef struct {
  * [total_q, H, D]) and n = cu_k[b+1] - cu_k[b] keys (k, v bf16 [total_k, H_kv, D]), and
  *   out[i, h] = sum_j w_ij v[j, h'],  w = softmax over j of scale * q[i, h] . k[j, h'],
  * over all n keys, or with `causal` over j <= i + n - m (the queries are the last m positions).
- * A row that its mask leaves no key is 0. scale > 0; 0 stands for 1 / sqrt(D). What is not
- * finite in keys that a row's mask leaves out does not reach the row. */
+ * A row that its mask leaves no key is 0. 0 < scale <= 2.3e38 (its product with log2(e) is formed in
+ * f32); 0 stands for 1 / sqrt(D). What is not finite in keys that a row's mask leaves out does not
+ * reach the row. */
 MB_API mb_status mb_attention_varlen(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                                      int64_t ldv, int64_t total_q, int64_t total_k, int H, int H_kv, int D,
                                      const int32_t* cu_q, const int32_t* cu_k, int n_seqs, int causal, float scale,

@@ -931,7 +931,7 @@ mb_status mb_attention_paged(const void* q, int64_t ldq, const mb_kv_cache* cach
   if (s == MB_OK) s = check_kv_table(table, ld_table, table_width, n_seqs);
   if (s == MB_OK) s = check_heads(n_seqs, H, cache->n_kv_heads, cache->head_dim);
   if (s != MB_OK) return s;
-  MB_CHECK(scale >= 0.f && scale <= 3.0e38f, MB_ERR_INVALID, "scale must be positive and finite (0: 1 / sqrt(D))");
+  MB_CHECK(scale >= 0.f && scale <= 2.3e38f, MB_ERR_INVALID, "scale must be positive, at most 2.3e38 (0: 1 / sqrt(D))");
   if (n_seqs == 0) return MB_OK;
   const int D = cache->head_dim;
   MB_CHECK(kv_lens, MB_ERR_INVALID, "kv_lens is NULL");

@@ -680,7 +680,7 @@ extern "C" mb_status mb_attention_varlen(const void* q, int64_t ldq, const void*
   MB_CHECK(total_q >= 0 && total_q < (1LL << 30) && total_k >= 0 && total_k < (1LL << 30), MB_ERR_INVALID,
            "total_q and total_k must be from 0 to 2^30 - 1");
   MB_CHECK(n_seqs >= 0 && n_seqs < (1 << 24), MB_ERR_INVALID, "n_seqs must be from 0 to 2^24 - 1");
-  MB_CHECK(scale >= 0.f && scale <= 3.0e38f, MB_ERR_INVALID, "scale must be positive and finite (0: 1 / sqrt(D))");
+  MB_CHECK(scale >= 0.f && scale <= 2.3e38f, MB_ERR_INVALID, "scale must be positive, at most 2.3e38 (0: 1 / sqrt(D))");
   if (total_q == 0 || n_seqs == 0) return MB_OK;
   MB_CHECK(cu_q && cu_k, MB_ERR_INVALID, "cu_q or cu_k is NULL");
   auto rows_ok = [](const void* x, int64_t ld, int64_t width) {

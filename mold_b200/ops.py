@@ -359,7 +359,7 @@ def _scale(scale):
         return 0.0
     if not scale > 0:
         raise ValueError(f"scale must be positive, got {scale}")
-    return float(scale)
+    return max(float(scale), 2.0 ** -126)  # a smaller one may be 0 in 32 bits, which stands for the default
 
 
 def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None):
