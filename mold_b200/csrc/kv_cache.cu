@@ -335,7 +335,7 @@ mb_status check_kv_cache(const mb_kv_cache* c) {
            "page_size must be a power of two from 16 to 256");
   MB_CHECK(c->n_kv_heads > 0 && c->n_kv_heads <= 65535 && c->n_pages > 0 && c->n_pages < (1LL << 31), MB_ERR_INVALID,
            "cache sizes must be positive, n_pages below 2^31 and n_kv_heads below 65536");
-  MB_CHECK(c->n_pages < (1LL << 31) / ((int64_t)c->n_kv_heads * c->page_size), MB_ERR_INVALID,
+  MB_CHECK(c->n_pages <= ((1LL << 31) - 1) / ((int64_t)c->n_kv_heads * c->page_size), MB_ERR_INVALID,
            "n_pages * n_kv_heads * page_size must be below 2^31");
   MB_CHECK(c->k && c->v, MB_ERR_INVALID, "cache k or v is NULL");
   MB_CHECK(((uintptr_t)c->k & 15) == 0 && ((uintptr_t)c->v & 15) == 0, MB_ERR_INVALID,

@@ -4,7 +4,7 @@ import torch
 
 import mold_b200 as mb
 from mold_b200 import _lib, ops
-from tests.test_text_ops import INVALID, NOT_READY, paged, varlen
+from tests.test_text_ops import INVALID, NOT_READY, cache, paged, read, varlen, write
 
 
 def test_a_small_scale_does_not_become_the_default():
@@ -39,3 +39,14 @@ def test_tiny_scales_weigh_all_keys_alike(cuda, scale):
     cache.write(k, v, table, lens, cu=cu)
     out = mb.attention_paged(q[:1], cache, table, lens, scale=scale)
     assert ((out.double() - mean).abs() <= 2.0 ** -8 * mean.abs() + 2.0 ** -16 * size).all()
+
+
+@pytest.mark.parametrize("heads,page", [(3, 16), (7, 64), (1, 16), (5, 256)])
+def test_every_cache_below_2_to_the_31_rows_is_taken(heads, page):
+    most = ((1 << 31) - 1) // (heads * page)
+    for call in (paged, write, read):
+        kw = {"H": 2 * heads, "ldq": 256 * heads, "ldo": 256 * heads} if call is paged else dict(ldk=128 * heads,
+                                                                                                 ldv=128 * heads)
+        if not torch.cuda.is_available():
+            assert call(cache=cache(n_pages=most, n_kv_heads=heads, page_size=page), **kw) == NOT_READY
+        assert call(cache=cache(n_pages=most + 1, n_kv_heads=heads, page_size=page), **kw) == INVALID
