@@ -411,7 +411,12 @@ MB_API mb_status mb_flux_lora_merge(mb_flux* m, const char* name, int64_t row_of
  * given sizes are neither read nor written, and a page number outside the cache that a call
  * needed raises MB_DEV_BAD_PAGE in the device status word (mb_device_status). mb_init must have
  * been called on the device (else MB_ERR_NOT_READY). Nothing is allocated; every call may be
- * captured into a CUDA graph, and its scratch is the caller's. */
+ * captured into a CUDA graph, and its scratch is the caller's.
+ * Numerics of both attentions: scores, softmax statistics and sums in f32. The weights are rounded
+ * to bf16 (over 8-bit caches to f16, with the value's scale) for their product with the values.
+ * Over int8 caches a query is taken to 1 / 65278 of its row's largest magnitude (a row below 2^-100
+ * as 0), over e4m3 caches to 2^-25. The weights' sum is divided out last: n values of 2^119 / n and
+ * more may add up to infinity. */
 
 enum { MB_DEV_BAD_PAGE = 0x400 };
 

@@ -2,19 +2,19 @@
 // with a scale a row), split over the cached length and joined.
 //
 // Work is counted in tiles of kTileKeys keys of one unit = (sequence, key head, up to 16 of the query
-// heads that read it), and kUnitCost for a unit's own expense. All units in a row are cut into runs of
-// equal cost, one for each block of a grid that fills the SMs, so blocks end together however far the
-// lengths lie apart. A block's part of a
-// unit that it does not hold whole goes to the workspace as (max, sum, unnormalised output); k_join adds
-// a unit's parts in the order of the blocks.
+// heads that read it), and Shape::UNIT_COST for a unit's own expense. All units in a row are cut into
+// runs of equal cost, one for each block of a grid that fills the SMs, so blocks end together however far
+// the lengths lie apart. A block's part of a unit that it does not hold whole goes to the workspace as
+// (max, sum, unnormalised output); k_join adds a unit's parts in the order of the blocks.
 //
 // One warp of a block walks the run and keeps a ring of tiles in flight: page numbers, one TMA box of 16 to
 // 64 keys x 128 bytes after the other (keys, values; 128-byte swizzle), scales and the unit's queries, all
 // landing on the stage's mbarrier. It runs ahead over the borders of units, so a batch of short
-// sequences keeps memory as busy as a long one. Four warps take 16 keys of a tile each: q k^T and p v as
-// warp products (query heads as rows; at one token a row there is too little arithmetic for more). Which
-// k index of q k^T stands for which channel is free as long as both operands agree, so a lane reads 16
-// contiguous bytes of a key row. Scores, maximum, sum and output stay in f32.
+// sequences keeps memory as busy as a long one. Four warps take 16 keys of a tile each: scores and outputs
+// as warp products (at one token a sequence there is too little arithmetic for more). Which depth index of
+// the scores' product stands for which channel is free as long as both operands agree, so a lane reads 16
+// contiguous bytes of a key row. Scores, maximum, sum and output stay in f32; over a bf16 cache the weights
+// are rounded to bf16 for the product with the values (2^-8 of each; their sum takes them unrounded).
 //
 // Both products are formed transposed: keys (16) are the rows of K q^T and channels those of V^T p^T, with
 // 8 query heads as columns, so that no row of a product is idle where few heads share a key head. A
@@ -23,7 +23,8 @@
 // 8-bit caches: the products run on the codes, the key's scale multiplies the score, the value's scale
 // the weight.
 //   int8 scores need no conversion of codes: a query becomes s (256 h + l) with int8 digits h and l, off by
-//   at most 2^-16 of its row's largest magnitude, and the integer sums are exact.
+//   at most 1 / 65278 of its row's largest magnitude (half a step of 1 / 32639), and the integer sums are
+//   exact. A row below 2^-100 counts as 0.
 //   e4m3 scores: codes to f16, which holds every code, with the query row times a power of two in f16 (off
 //   by at most 2^-25 of the row's largest magnitude). The 8-bit float product is no help here: it measured
 //   as many instructions as the conversion.

@@ -17,8 +17,8 @@
 //             finite before the product reads them; rows that may see such a value add it at the end (a
 //             slow path that ordinary data never takes).
 //   warps 4-7 softmax, one thread a query row (= TMEM lane), as in K4 (attention.cu): 64 scores in
-//             registers, P written back over S as bf16, lazy rescale of O. Only blocks that cross a row's
-//             limit are masked.
+//             registers, P written back over S as bf16 (2^-8 of each weight: the products' type; the sum of
+//             weights takes them unrounded), lazy rescale of O. Only blocks that cross a row's limit are masked.
 // TMEM (256 columns a block): S [0, 128) in halves of 64, O [128, 128 + D).
 //
 // Bound by the softmax's chain on one thread a row (its exponentials alone take the tensor core's time)
