@@ -1,4 +1,4 @@
-// Device helpers of the tcgen05 attention kernels (attention.cu, attn_varlen.cu).
+// Device helpers of the tcgen05 attention kernels (attention.cu, attn_varlen.cu); the packed arithmetic serves kv_cache.cu too.
 #pragma once
 #include "common.cuh"
 

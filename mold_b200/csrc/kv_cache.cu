@@ -11,6 +11,7 @@
 // bytes (40.4 against 39.9).
 #include <string>
 
+#include "attn_util.cuh"
 #include "common.cuh"
 #include "internal.h"
 #include "kv_cache.cuh"
@@ -51,22 +52,14 @@ MB_DEV Span seq_of(const int32_t* cu, const int32_t* per_seq, int n, int64_t t) 
   return s;
 }
 
-MB_DEV uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1,%2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
+using attn::add2;
+using attn::pk2;
+using attn::up2;
 MB_DEV uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-MB_DEV uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-MB_DEV void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0,%1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 MB_DEV uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -136,27 +129,27 @@ MB_DEV void encode_row(const uint4 (&x)[kHalves], uint2 (&out)[kHalves], float& 
     r = 0.f;
     scale = top < 0x0d800000u ? 0.f : __uint_as_float(0x7fc00000u);
   }
-  const uint64_t r2 = pack2(r, r);
+  const uint64_t r2 = pk2(r, r);
 #pragma unroll
   for (int i = 0; i < kHalves; i++) {
     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     uint32_t o[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      uint64_t a = mul2(pack2(bf16_lo(w[2 * j]), bf16_hi(w[2 * j])), r2);
-      uint64_t b = mul2(pack2(bf16_lo(w[2 * j + 1]), bf16_hi(w[2 * j + 1])), r2);
+      uint64_t a = mul2(pk2(bf16_lo(w[2 * j]), bf16_hi(w[2 * j])), r2);
+      uint64_t b = mul2(pk2(bf16_lo(w[2 * j + 1]), bf16_hi(w[2 * j + 1])), r2);
       float y0, y1, y2, y3;
       if (CODES == MB_KV_I8) {
         // |y| <= 127 (1 + 2^-23); adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the
         // low byte (the conversion instruction runs at a quarter of the rate). Scalar additions: a packed one after the
         // packed product came out as one fused operation, without the product's rounding, and took ties the wrong way.
-        unpack2(a, y0, y1), unpack2(b, y2, y3);
+        up2(a, y0, y1), up2(b, y2, y3);
         const uint32_t v0 = __float_as_uint(__fadd_rn(y0, 12582912.f)), v1 = __float_as_uint(__fadd_rn(y1, 12582912.f));
         const uint32_t v2 = __float_as_uint(__fadd_rn(y2, 12582912.f)), v3 = __float_as_uint(__fadd_rn(y3, 12582912.f));
         o[j] = __byte_perm(__byte_perm(v0, v1, 0x0040), __byte_perm(v2, v3, 0x0040), 0x5410);
       } else {
         uint16_t lo, hi;
-        unpack2(a, y0, y1), unpack2(b, y2, y3);
+        up2(a, y0, y1), up2(b, y2, y3);
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y1), "f"(y0));
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y3), "f"(y2));
         o[j] = (uint32_t)lo | ((uint32_t)hi << 16);
@@ -237,14 +230,14 @@ MB_DEV uint64_t decode2(uint32_t w, int i) {
   if (CODES == MB_KV_I8) {
     // byte c + 128 in the last place of 2^23
     const uint32_t u = w ^ 0x80808080u;
-    return add2(pack2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + 2 * i)),
+    return add2(pk2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + 2 * i)),
                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7651 + 2 * i))),
-                pack2(-8388736.f, -8388736.f));
+                pk2(-8388736.f, -8388736.f));
   }
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (16 * i))));
   const float2 f = __half22float2(*(const __half2*)&h);
-  return pack2(f.x, f.y);
+  return pk2(f.x, f.y);
 }
 
 template <int CODES>
@@ -272,13 +265,13 @@ MB_DEV void load_row(Held<CODES>& r, const void* base, const float* scales, int6
 template <int CODES>
 MB_DEV uint4 decode_row(const Held<CODES>& r, int j) {
   if (CODES == MB_KV_BF16) return r.x[j];
-  const uint64_t s2 = pack2(r.s, r.s);
+  const uint64_t s2 = pk2(r.s, r.s);
   uint32_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     // f32 product, then one rounding to bf16
     float a, b;
-    unpack2(mul2(decode2<CODES>(i < 2 ? r.x[j].x : r.x[j].y, i & 1), s2), a, b);
+    up2(mul2(decode2<CODES>(i < 2 ? r.x[j].x : r.x[j].y, i & 1), s2), a, b);
     o[i] = pack_bf16x2(a, b);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
