@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CODES, D, WIDE>::BLOCKS)
   wait_before();
   auto length = [&](int b) -> int64_t {
     if (b >= p.n_seqs) return 0;
-    const int64_t n = __ldg(p.lens + b);
+    const int64_t n = p.lens[b];
     return n < 0 ? 0 : n < cap ? n : cap;
   };
   auto tiles_of = [&](int64_t len) { return (len + kTileKeys - 1) / kTileKeys; };
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) k_join(const Params p) {
   const int b = u / p.units_per_seq, unit = u - b * p.units_per_seq;
   const int hk = unit / p.q_tiles, qt = unit - hk * p.q_tiles;
   if (r >= p.G - qt * kRows || p.table_width == 0) return;
-  const int len = __ldg(p.lens + b);
+  const int len = p.lens[b];
   const Part part = p.parts[u];
   if (len <= 0 || part.pieces <= 1) return;
   // left by another call where this one gave up a wait, or lengths changed under it

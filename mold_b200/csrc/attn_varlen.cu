@@ -113,10 +113,10 @@ MB_DEV bool find_work(const Params& p, int idx, int span, Work& w) {
     const int b = base + lane;
     int q0 = 0, m = 0, k0 = 0, n = 0;
     if (b < p.n_seqs) {
-      q0 = clampq(__ldg(p.cu_q + b));
-      m = max(0, clampq(__ldg(p.cu_q + b + 1)) - q0);
-      k0 = clampk(__ldg(p.cu_k + b));
-      n = max(0, clampk(__ldg(p.cu_k + b + 1)) - k0);
+      q0 = clampq(p.cu_q[b]);
+      m = max(0, clampq(p.cu_q[b + 1]) - q0);
+      k0 = clampk(p.cu_k[b]);
+      n = max(0, clampk(p.cu_k[b + 1]) - k0);
     }
     int x = (m + span - 1) / span;
 #pragma unroll
@@ -151,7 +151,7 @@ MB_DEV bool find_slot(const Params& p, int idx, int span, Work& w) {
 #pragma unroll 1
   while (n > 32) {
     const int step = (n + 31) >> 5, at = lane * step, b = lo + (at < n ? at : 0);
-    const unsigned le = __ballot_sync(0xffffffffu, at < n && clampq(__ldg(p.cu_q + b)) / span + b <= idx);
+    const unsigned le = __ballot_sync(0xffffffffu, at < n && clampq(p.cu_q[b]) / span + b <= idx);
     const int k = max(__popc(le), 1) - 1;  // le is a run of ones from bit 0
     lo += k * step;
     n = min(step, n - k * step);
@@ -159,10 +159,10 @@ MB_DEV bool find_slot(const Params& p, int idx, int span, Work& w) {
   const int b = lo + lane;
   int q0 = 0, m = 0, k0 = 0, nk = 0;
   if (lane < n) {
-    q0 = clampq(__ldg(p.cu_q + b));
-    m = max(0, clampq(__ldg(p.cu_q + b + 1)) - q0);
-    k0 = clampk(__ldg(p.cu_k + b));
-    nk = max(0, clampk(__ldg(p.cu_k + b + 1)) - k0);
+    q0 = clampq(p.cu_q[b]);
+    m = max(0, clampq(p.cu_q[b + 1]) - q0);
+    k0 = clampk(p.cu_k[b]);
+    nk = max(0, clampk(p.cu_k[b + 1]) - k0);
   }
   const int first = q0 / span + b;
   const int src = max(__popc(__ballot_sync(0xffffffffu, lane < n && first <= idx)), 1) - 1;

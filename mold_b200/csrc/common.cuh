@@ -90,7 +90,8 @@ MB_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
 // wait_before() ahead of its first access to global memory. 1 to 1.5 us a launch (cache write and read, 40 sequences, e4m3:
 // 28.8 -> 25.3 us); letting the next one start before this one's blocks end gained nothing more. The one before may be any
 // kernel of the stream, and may let this one's blocks in while blocks of its own still run: so nothing that those could wait
-// for (tensor memory above all) is held across the wait.
+// for (tensor memory above all) is held across the wait. Nor may such a kernel load through the read-only path (__ldg,
+// ld.global.nc): what it reads may still be written after it has started, which that path takes for impossible.
 MB_DEV void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <class... P>

@@ -35,19 +35,19 @@ MB_DEV Span seq_of(const int32_t* cu, const int32_t* per_seq, int n, int64_t t) 
   int lo = 0;
   while (n > 32) {
     const int step = (n + 31) >> 5, at = lane * step;
-    const unsigned le = __ballot_sync(0xffffffffu, at < n && __ldg(cu + lo + (at < n ? at : 0)) <= t);
+    const unsigned le = __ballot_sync(0xffffffffu, at < n && cu[lo + (at < n ? at : 0)] <= t);
     const int k = max(__popc(le), 1) - 1;  // le is a run of ones from bit 0
     lo += k * step;
     n = min(step, n - k * step);
   }
-  const int edge = lane <= n ? __ldg(cu + lo + lane) : 0;
-  const int value = per_seq && lane < n ? __ldg(per_seq + lo + lane) : 0;
+  const int edge = lane <= n ? cu[lo + lane] : 0;
+  const int value = per_seq && lane < n ? per_seq[lo + lane] : 0;
   const int k = max(__popc(__ballot_sync(0xffffffffu, lane < n && edge <= t)), 1) - 1;
   Span s;
   s.b = lo + k;
   s.c0 = __shfl_sync(0xffffffffu, edge, k);
   s.c1 = __shfl_sync(0xffffffffu, edge, (k + 1) & 31);
-  if (k == 31) s.c1 = __ldg(cu + lo + 32);
+  if (k == 31) s.c1 = cu[lo + 32];
   s.value = __shfl_sync(0xffffffffu, value, k);
   return s;
 }
@@ -77,8 +77,8 @@ MB_DEV int64_t first_token(int heads, int& h) {
 // On to the sequence that holds t, at or behind the present one.
 MB_DEV void advance(Span& s, const int32_t* cu, const int32_t* per_seq, int n, int64_t t) {
   while (t >= s.c1 && s.b + 1 < n) {
-    s.b++, s.c0 = s.c1, s.c1 = __ldg(cu + s.b + 1);
-    if (per_seq) s.value = __ldg(per_seq + s.b);
+    s.b++, s.c0 = s.c1, s.c1 = cu[s.b + 1];
+    if (per_seq) s.value = per_seq[s.b];
   }
 }
 
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_write(const WriteParams p) {
       if (t >= seq.c0 && t < seq.c1) pos = seq.value - (seq.c1 - t);
     }
   } else if (here) {
-    pos = (int64_t)__ldg(p.lens + seq.b) - 1;
+    pos = (int64_t)p.lens[seq.b] - 1;
   }
   if (pos >= 0) dst = row_of(p.c, p.table + (int64_t)seq.b * p.ld_table, p.table_width, pos, h, p.status);
   if (CODES == MB_KV_BF16) {
@@ -260,7 +260,7 @@ MB_DEV void load_row(Held<CODES>& r, const void* base, const float* scales, int6
       r.x[j].x = c.x, r.x[j].y = c.y;
     }
   }
-  if (CODES != MB_KV_BF16 && src >= 0) r.s = __ldg(scales + src);
+  if (CODES != MB_KV_BF16 && src >= 0) r.s = scales[src];
 }
 template <int CODES>
 MB_DEV uint4 decode_row(const Held<CODES>& r, int j) {

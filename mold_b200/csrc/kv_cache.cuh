@@ -19,7 +19,7 @@ struct Cache {
 // the device status) where the position has no page or its page is not one of the cache's.
 MB_DEV int64_t row_of(const Cache& c, const int32_t* table, int table_width, int64_t pos, int h, int* status) {
   const int64_t at = pos >> c.page_log2;
-  const int64_t page = at < table_width ? (int64_t)__ldg(table + at) : -1;
+  const int64_t page = at < table_width ? (int64_t)table[at] : -1;
   if (page < 0 || page >= c.n_pages) {
     atomicExch(status, kDevBadPage);
     return -1;

@@ -53,6 +53,15 @@ def test_nothing_before_the_wait(what):
         assert what not in before, f"{f}: {name} has {what} ahead of wait_before()"
 
 
+def test_no_loads_through_the_read_only_path():
+    """Its data may not change while a kernel lives, and a kernel that is launched close lives while the one before it
+    writes. In the kernels' files, headers for them included."""
+    files = {k[0] for k in close_kernels()} | {"kv_cache.cuh", "attn_util.cuh"}
+    for f in files:
+        s = re.sub(r"//[^\n]*", "", sources()[f])
+        assert "__ldg" not in s and ".nc." not in s and "__restrict__" not in s, f
+
+
 def body(name):
     return next(k[2] for k in kernels() if k[1] == name)
 
