@@ -30,7 +30,8 @@ def batch(kind):
         ms = [1] * 2049
     else:
         ms = [r.choice([0, 1, 300]) if i % 97 == 0 else 2 for i in range(1025)]
-    return ms, [m + r.choice([0, 0, 3, 70]) if m else r.choice([0, 4]) for m in ms]
+    # keys: as many, a few more (a prefix), or now and then none at all
+    return ms, [r.choice([0, m, m, m + 3, m + 70]) if m else r.choice([0, 4]) for m in ms]
 
 
 @pytest.mark.parametrize("kind", ["short", "mostly_empty", "one_token", "lopsided"])
