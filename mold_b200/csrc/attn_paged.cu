@@ -33,9 +33,10 @@
 //   be any finite numbers, of either sign.
 // Converting codes to bf16 instead kept the ALU pipe at 58 % and memory at 3.1 TB/s.
 //
-// Bound by HBM: 64 sequences of 64 to 4096 keys, 32 / 8 heads of 128, bf16: 50.9 us, 5.2 TB/s; 2 of 100001 to 131072, int8:
-// 87 us, 5.9 TB/s; 160 of 256 to 8192, 64 / 8 heads, e4m3: 146 us, 5.5 TB/s. A plain sum over as many bytes takes 51.0, 94.8 and
-// 139 us. More than 8 heads a key head over 8-bit caches are bound by the products' latency (16 heads of 128: 3.6 to 4.1 TB/s).
+// Bound by HBM, or nearly: 64 sequences of 64 to 4096 keys, 32 / 8 heads of 128, bf16: 51.1 us, 5.2 TB/s; 2 of 100001 to 131072,
+// int8: 88.9 us, 5.8 TB/s; 160 of 256 to 8192, 64 / 8 heads, e4m3: 152.9 us, 5.3 TB/s (at full clock 142.6; DRAM at 73 %, ALU pipe at
+// 50 %). Medians, timed in turn with a plain sum over as many bytes, which takes 48.0, 94.5 and 141.4 us. More than 8 heads a key
+// head over 8-bit caches are bound by the products' latency (16 heads of 128: 3.6 to 4.1 TB/s).
 #include <math.h>
 
 #include <string>

@@ -22,8 +22,9 @@
 // TMEM (256 columns a block): S [0, 128) in halves of 64, O [128, 128 + D).
 //
 // Bound by the softmax's chain on one thread a row (its exponentials alone take the tensor core's time)
-// and, in long runs, by the board's power. One prompt of 8201 tokens, 32 / 8 heads of 128: 539 us, 1022 TFLOP/s
-// (0.62 of the measured burst rate); 24 prompts of 32 to 2048 tokens: 205 us. Measured and not kept: two softmax
+// and, in long runs, by the board's power. One prompt of 8201 tokens, 32 / 8 heads of 128: 547 us, 1008 TFLOP/s
+// (0.61 of the measured burst rate; at full clock 478 us); 24 prompts of 32 to 2048 tokens: 213 us (184). Heads of 64, one
+// prompt of 8201: 401 us. Measured and not kept: two softmax
 // groups on alternate blocks (568 against 542 us on the long prompt: 16 softmax warps slow the issuer),
 // 128-key score products with two groups (607 us: one S buffer), K4's share of polynomial exponentials
 // (618 against 556 us), the output by TMA (no stage is free under the next tile's loads), a tile's output after

@@ -3,8 +3,8 @@
 //
 // A group of head_dim / 16 threads owns a (token, head) row of k and the same row of v, two times 16 bytes
 // of bf16 a thread; the groups of a warp work on neighbouring tokens and search for the sequence together,
-// while the rows are on their way. 11k rows of 8 x 128 written and 25k read, int8: 38.8 us, 216 MB in and out or
-// 5.6 TB/s. Of these some 135 MB pass HBM (3.5 TB/s), the codes and part of the output stay in L2: no single
+// while the rows are on their way. 11k rows of 8 x 128 written and 25k read, int8: 39.6 us, 216 MB in and out or
+// 5.5 TB/s. Of these some 135 MB pass HBM (3.5 TB/s), the codes and part of the output stay in L2: no single
 // unit is full (issue slots 60 to 65 %, ALU pipe 53 to 58 %), and two short launches start and end. Instructions
 // count, hence packed f32 arithmetic and no integer conversions or divisions (55 us with them). More rows a
 // thread or larger blocks lose (2 rows: 41.2, 4: 48 us; a generation step 6.1 and 9.6 against 4.8 us), and so do accesses of 32
