@@ -51,6 +51,7 @@ struct Params {
   int n_seqs;
   int64_t total_q, total_k;
   int Hkv, G, TQ, causal;
+  unsigned blocks;
   float scale_log2;
   const __nv_bfloat16* v;
   int64_t ldv;
@@ -655,9 +656,7 @@ cudaError_t launch(const Params& p, const void* q, int64_t ldq, const void* k, i
     if (e != cudaSuccess) return e;
     attr_done[dev & 63] = 1;
   }
-  const int64_t blocks = (p.total_q / p.TQ + p.n_seqs) * p.Hkv;  // each sequence rounds up once
-  if (blocks >= (1LL << 31)) return cudaErrorInvalidConfiguration;
-  return launch_close(k_attention_varlen<D, MANY>, dim3((unsigned)blocks), kThreads, Smem<D>::kBytes, st, 1, tq, tk, tv, p);
+  return launch_close(k_attention_varlen<D, MANY>, dim3(p.blocks), kThreads, Smem<D>::kBytes, st, 1, tq, tk, tv, p);
 }
 
 template <int D>
@@ -691,6 +690,8 @@ extern "C" mb_status mb_attention_varlen(const void* q, int64_t ldq, const void*
            "q and out must be 16-byte aligned with row strides of at least H * D, multiples of 8");
   MB_CHECK(total_k == 0 || (rows_ok(k, ldk, (int64_t)H_kv * D) && rows_ok(v, ldv, (int64_t)H_kv * D)), MB_ERR_INVALID,
            "k and v must be 16-byte aligned with row strides of at least H_kv * D, multiples of 8");
+  const int64_t blocks = (total_q / (128 / (H / H_kv)) + n_seqs) * H_kv;  // each sequence rounds up once
+  MB_CHECK(blocks < (1LL << 31), MB_ERR_INVALID, "too many tiles for one launch");
   MB_CHECK(device_status_ready(), MB_ERR_NOT_READY, "call mb_init on this device first");
   varlen::Params p;
   p.cu_q = cu_q;
@@ -701,6 +702,7 @@ extern "C" mb_status mb_attention_varlen(const void* q, int64_t ldq, const void*
   p.Hkv = H_kv;
   p.G = H / H_kv;
   p.TQ = 128 / p.G;
+  p.blocks = (unsigned)blocks;
   p.causal = causal != 0;
   p.scale_log2 = (float)((scale > 0.f ? (double)scale : 1.0 / sqrt((double)D)) * 1.4426950408889634);
   p.v = (const __nv_bfloat16*)v;

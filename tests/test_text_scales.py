@@ -50,3 +50,11 @@ def test_every_cache_below_2_to_the_31_rows_is_taken(heads, page):
         if not torch.cuda.is_available():
             assert call(cache=cache(n_pages=most, n_kv_heads=heads, page_size=page), **kw) == NOT_READY
         assert call(cache=cache(n_pages=most + 1, n_kv_heads=heads, page_size=page), **kw) == INVALID
+
+
+def test_more_tiles_than_a_launch_has_blocks_are_refused():
+    """As an argument out of range, not as a failure of the device."""
+    big = dict(H=128, Hkv=128, D=64, ldq=128 * 64, ldk=128 * 64, ldv=128 * 64, ldo=128 * 64)
+    assert varlen(n=(1 << 24) - 1, tq=1 << 20, **big) == INVALID
+    if not torch.cuda.is_available():
+        assert varlen(n=(1 << 24) - 1, **{**big, "H": 64, "Hkv": 64}) == NOT_READY
